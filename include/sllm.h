@@ -224,6 +224,101 @@ int sllm_k_attn_decode_static(sllm_engine* e, uint32_t layer, uint32_t n_tok, co
                               const int32_t* d_tok_slot, const int32_t* d_tok_pos, uint32_t n_splits, float* d_out,
                               void* stream);
 
+/* ---- the 8-bit KV cache: single kernels, device pointers in and out -----------------------------
+ * No counterpart in the reference (it keeps no KV cache).  Operators of a paged cache that holds K and V as int8 with one
+ * fp32 scale for each block of 16 positions, head, and K or V (a stored integer q stands for q * scale): half the bytes
+ * of the engine's bf16 cache.  They are independent of an engine: all memory is the caller's, nothing is allocated, nothing
+ * is kept between calls, and grouped heads (kv_heads < n_heads) are supported.  A serving step is
+ * sllm_k_block_tables, then per layer sllm_k_kv8_append and sllm_k_attn_kv8, all asynchronous on `stream`
+ * (a cudaStream_t as void*, NULL = the default stream), with no host round trip between them; the whole step can be captured
+ * into a CUDA graph (lists padded to a fixed length, see below).
+ *
+ * Every pointer must be device memory of the calling thread's current device (SLLM_ERR_INVALID otherwise); error texts are read
+ * with sllm_last_error(NULL).  Calls may overlap on the GPU when the memory they write is neither written nor read by another of
+ * them: a workspace belongs to one call in flight, and two graphs that may run at the same time need one each.
+ * What the device finds in lists and tables never leads outside the arrays: a slot, sequence or page outside them is
+ * skipped as said at each call. */
+
+/* One layer of the cache.  A slot is page * 64 + (position % 64). */
+typedef struct {
+    int8_t* pages;             /* [n_pages][kv_heads][2][64][head_dim], [2]: K, V; 16-byte aligned                */
+    float* scales;             /* [n_pages][kv_heads][2][4], 16-byte aligned                                       */
+    uint64_t n_pages;          /* 1 .. 2^31 - 1                                                                    */
+    uint32_t kv_heads, head_dim;   /* head_dim 16, 32, 64 or 128                                                   */
+} sllm_kv8_layer;
+
+enum { SLLM_ROWS_BF16 = 0, SLLM_ROWS_F32 = 1 };
+
+/* Block tables, token lists and slot maps of a step, from the lengths of the sequences before and after it.  Sequence i holds
+ * len_before[i] positions in pages table[i][0 .. ceil(len_before[i] / 64)) and is to hold len_after[i]:
+ *   longer:   its new positions become list entries, and pages for them are taken from the front of the ring of free pages,
+ *             in the order of the sequences;
+ *   shorter:  (0 = it has ended) no entries; the pages it no longer needs go behind the ring's end, in that order.  They
+ *             can be taken from the next call on.
+ * Table entries behind a sequence's pages are left as they were.  Lists, for new position number t of the step, in the order of
+ * the sequences and positions: tok_seq[t], tok_pos[t] and slot_map[t]; entries behind the last are -1 up to max_tok, so that
+ * a graph captured for max_tok entries can be replayed for fewer.  cu_tok[i] is the number of entries before sequence i's.
+ * pool_in {first free entry of the ring, free pages, -, -}; pool_out the same after the call, the number of list
+ * entries, and a status: SLLM_OK; SLLM_ERR_CAPACITY (more pages or entries are needed than there are) or SLLM_ERR_INVALID (a length
+ * below 0 or above table_width * 64, or counters that contradict n_pages).  With a status other than SLLM_OK nothing is changed
+ * but that cu_tok is all 0 and the lists are all -1, which the calls below take as nothing to do. */
+typedef struct {
+    const int32_t *len_before, *len_after;    /* [n_seq]                                                           */
+    int32_t* table;                           /* [n_seq][table_width], in and out                                  */
+    int32_t* ring;                            /* [n_pages], in and out                                             */
+    const int64_t* pool_in;                   /* [4]                                                               */
+    int64_t* pool_out;                        /* [4], not pool_in                                                  */
+    int32_t* cu_tok;                          /* [n_seq + 1]                                                       */
+    int32_t *tok_seq, *tok_pos;               /* [max_tok]                                                         */
+    int64_t* slot_map;                        /* [max_tok]                                                         */
+    uint64_t n_pages;
+    uint32_t n_seq, table_width, max_tok;     /* n_seq 1 .. 8192                                                   */
+} sllm_block_tables;
+int sllm_k_block_tables(const sllm_block_tables* a, void* stream);
+
+/* Rows of K and V into the cache, row t to slot_map[t] (outside the pool, -1 for instance: skipped).  A row is
+ * kv_heads * head_dim consecutive elements (head h from h * head_dim on), rows k_stride and v_stride elements apart, of the
+ * fused projection's output for instance.  A block of 16 positions gets the scale
+ *   s = max(s_before, max |x| / 127)      s_before: its scale so far, 0 when its first position is among the rows
+ * and its rows become rint(x / s), half to even; rows that it held below them become rint(q * s_before / s) when s grew.  What it
+ * held above them is given up.  Rows of a sequence must be consecutive entries in order (as sllm_k_block_tables writes them): two
+ * runs of entries must not fall into one block.  A value that is not finite makes the scale, and so what the
+ * block stands for, NaN until its first position is written again. */
+typedef struct {
+    const void *k, *v;
+    const int64_t* slot_map;                  /* [n_tok]                                                           */
+    uint64_t k_stride, v_stride;              /* elements                                                          */
+    uint32_t n_tok, dtype;                    /* SLLM_ROWS_*                                                       */
+} sllm_kv8_rows;
+int sllm_k_kv8_append(const sllm_kv8_layer* c, const sllm_kv8_rows* r, void* stream);
+/* The rows that the cache stands for, q * s, in r->dtype: r->k and r->v are written, rows of slots outside the pool with zeros. */
+int sllm_k_kv8_read(const sllm_kv8_layer* c, const sllm_kv8_rows* r, void* stream);
+
+/* Causal attention over the cache: token t, of sequence tok_seq[t], attends the positions 0 .. tok_pos[t] of that sequence
+ * (its own included: append first).  n_heads is a multiple of kv_heads; query head h attends kv head h / (n_heads / kv_heads).
+ * Softmax in fp32 and the integers of the cache exactly; fp32 rows keep fp32 accuracy.
+ * A token with tok_seq outside 0 .. n_seq - 1 is skipped, its output row left as it was; one with tok_pos < 0 gets zeros.  A
+ * page outside the pool is not attended, and *status (when given, an int32 that the call never clears) becomes SLLM_ERR_INVALID.
+ * max_new: the most entries that one sequence has; max_len: the most positions that one has.  They choose between kernels and how
+ * the keys are cut; 0 = not known; a wrong value costs time, not results.  cu_tok (NULL allowed: then every token is taken
+ * alone) says that entries cu_tok[i] .. cu_tok[i + 1] - 1 are sequence i's, with the table's row i; it is used when max_new != 1. */
+typedef struct {
+    const void* q;                            /* [n_tok], rows of n_heads * head_dim elements                      */
+    void* out;                                /* the same; may not overlap q                                       */
+    uint64_t q_stride, out_stride;            /* elements                                                          */
+    const int32_t* table;                     /* [n_seq][table_width]                                              */
+    const int32_t *tok_seq, *tok_pos;         /* [n_tok]                                                           */
+    const int32_t* cu_tok;                    /* [n_seq + 1] or NULL                                               */
+    int32_t* status;                          /* or NULL                                                           */
+    uint32_t n_tok, n_seq, table_width, n_heads;
+    uint32_t max_new, max_len;
+    uint32_t dtype;                           /* SLLM_ROWS_*, of q and out                                         */
+    float scale;                              /* of the scores; 0 = 1 / sqrt(head_dim)                             */
+} sllm_kv8_attn;
+/* Bytes of workspace that this call needs on the current device (0: none). */
+int sllm_k_attn_kv8_workspace(const sllm_kv8_layer* c, const sllm_kv8_attn* a, uint64_t* bytes);
+int sllm_k_attn_kv8(const sllm_kv8_layer* c, const sllm_kv8_attn* a, void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* ---- the KV cache of one slot, from and to the host --------------------------------------------
  * No counterpart in the reference (it keeps no KV cache; these rows are what its Attention::forward holds in k and
  * v after split_heads and rope, src/nn/attention.cpp:68-77, for the slot's positions).  Rows are HOST memory,

@@ -71,7 +71,8 @@ ABI_SYMBOLS = [
     "sllm_set_step_logits", "sllm_force_token", "sllm_truncate", "sllm_generate", "sllm_decode_loop", "sllm_k_attn_decode", "sllm_k_attn_decode_static",
     "sllm_eval_loss", "sllm_slot_assign", "sllm_slot_append", "sllm_slot_release", "sllm_get_finished", "sllm_num_live",
     "sllm_k_wait_probe", "sllm_kv_write", "sllm_kv_read", "sllm_decode_loop_timed",
-    "sllm_engine_make_current",
+    "sllm_engine_make_current", "sllm_k_block_tables", "sllm_k_kv8_append", "sllm_k_kv8_read", "sllm_k_attn_kv8_workspace",
+    "sllm_k_attn_kv8",
 ]
 
 

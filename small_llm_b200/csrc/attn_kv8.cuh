@@ -1,0 +1,433 @@
+// Attention over the 8-bit paged cache (kv8.cuh) for few query rows per sequence: decode, drafts, grouped heads, and the
+// general form for every type and size.
+//
+//   o = sum_j p_j vs_b(j) V_j / sum_j p_j,   p_j = exp(scale ks_b(j) (q . K_j) - m),   j <= position of the row
+//
+// with K_j, V_j the stored integers and ks, vs the scales of their blocks of 16 positions.  Only a block's scale touches an
+// integer product, so the products run on the integers themselves, which are exact in fp16: mma.sync m16n8k16 with eight
+// query rows (tokens x heads that share a kv head) as its rows 0..7, and fp32 accumulators.  Rows 8..15 carry what fp16
+// rounds away: q and p are split into a high and a low fp16 part (22 bits), both products come out in the same thread
+// and are added there.  q is first divided by a power of two so that its largest value is in [0.5, 1); p vs is divided by
+// vr, a power of two no smaller than the largest vs so far, which is carried like the running maximum m.  So fp32 queries
+// keep fp32 accuracy, at no more matrix instructions than one row costs.
+//
+// The kernel is bound by HBM: 2 head_dim bytes per cached position and kv head.  An int8 in the cache costs about 1.4
+// instructions on its way to the matrix unit (xor the sign, byte-permute under 0x64 = 1024 + x, subtract), a fraction of what a scalar
+// dot product would.  A block of threads takes one (row tile, kv head, chunk of the keys); each of its four warps takes every
+// fourth unit of 32 keys, through bulk copies of its own, three units ahead, and has its own running state; the states
+// are joined once.  Keys are cut into chunks when there are few rows; a second, small kernel joins the chunks.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "attn_stream.cuh"
+#include "kv8.cuh"
+
+namespace sllm {
+
+constexpr int kA8Warps = 4;
+constexpr int kA8Threads = kA8Warps * 32;
+constexpr int kA8Stages = 3;
+constexpr int kA8Unit = 32;            // keys per step of a warp: two blocks of 16
+constexpr int kA8Rows = 8;             // query rows of a tile
+
+struct Attn8Args {
+    Kv8View c;
+    const void* q; void* out;          // [n_tok][n_heads][hd], rows q_stride / out_stride elements apart
+    long long q_stride, out_stride;
+    const int* table;                  // [n_seq][width]
+    const int* tok_seq; const int* tok_pos;    // [n_tok]
+    const int* cu_tok;                 // [n_seq + 1], or null: every token is a tile of its own
+    int n_tok, n_seq, width, n_heads, group;   // group = n_heads / kv heads
+    int rows_heads;                    // heads of a tile (<= 8), head_tiles tiles cover a group
+    int head_tiles;
+    int rows_toks;                     // tokens of a tile
+    int chunk;                         // keys per chunk, a multiple of 64
+    int n_chunks;
+    int wide;                          // q and out rows are 16-byte aligned
+    float scale;
+    float* part;                       // n_chunks > 1: [n_tok][n_heads][n_chunks][hd] sums, then [..][2] (m in log2 units, l)
+    float* part_ml;
+    int* status;                       // optional
+};
+
+template <int HD> __host__ __device__ constexpr size_t attn8_smem() {
+    // per warp and stage: K rows, V rows, eight scales (64 bytes reserved)
+    return (size_t)kA8Warps * kA8Stages * (2 * kA8Unit * HD + 64);
+}
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// bytes 0, 1 (or 2, 3) of four excess-128 bytes as two halves: 0x64xx is 1024 + xx, minus 1152 leaves the signed value
+__device__ __forceinline__ uint32_t halves(uint32_t w, uint32_t sel) {
+    const uint32_t x = __byte_perm(w, 0x64646464u, sel);
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+// high and low fp16 parts of two floats
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    const float2 f = __half22float2(h);
+    lo = pack_half(a - f.x, b - f.y);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// smallest power of two >= x, for 0 <= x < infinity (0 for 0)
+__device__ __forceinline__ float pow2_above(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return __uint_as_float((u + 0x007fffffu) & 0x7f800000u);
+}
+// the row tile of a block: tokens [t0, t0 + n) of one sequence (n = 0: nothing to do)
+__device__ __forceinline__ int attn8_tile(const Attn8Args& a, int tile, int& t0, int& seq) {
+    if (!a.cu_tok) {
+        t0 = tile;
+        seq = a.tok_seq[tile];
+        return seq >= 0 && seq < a.n_seq ? 1 : 0;
+    }
+    // sequence i gets tile numbers from cu[i] / rows_toks + i on: at least as many as it needs, and found by a binary search
+    int lo = 0, hi = a.n_seq;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.cu_tok[mid] / a.rows_toks + mid <= tile) lo = mid; else hi = mid;
+    }
+    const int first = a.cu_tok[lo];
+    const int end = min(a.cu_tok[lo + 1], a.n_tok);
+    t0 = first + (tile - first / a.rows_toks - lo) * a.rows_toks;
+    seq = lo;
+    return first >= 0 && t0 >= 0 ? min(a.rows_toks, end - t0) : 0;
+}
+
+// chunks of a tile whose last row stands at `last`
+__device__ __forceinline__ int attn8_chunks(const Attn8Args& a, int last) { return min((last + a.chunk) / a.chunk, a.n_chunks); }
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
+    constexpr int KS = HD / 16;                  // k steps of the score product
+    constexpr int KB = HD / 4;                   // bytes of a key row per lane
+    constexpr int VB = HD / 8;                   // bytes of a value row per lane = column tiles of the output
+    constexpr uint32_t RUN = kA8Unit * HD;       // bytes of a unit's K (or V) rows
+    constexpr uint32_t STAGE = 2 * RUN + 64;
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    __shared__ __align__(8) unsigned long long bars[kA8Warps][kA8Stages];
+    __shared__ float s_m[kA8Warps][kA8Rows], s_l[kA8Warps][kA8Rows];
+    __shared__ int s_ok;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    if (tid == 0) {
+        for (int w = 0; w < kA8Warps; ++w)
+            for (int s = 0; s < kA8Stages; ++s) bar_init(as_smem(&bars[w][s]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        s_ok = 1;
+    }
+    pdl_launch_dependents();
+    pdl_wait();
+    int t0, seq;
+    const int n = attn8_tile(a, blockIdx.x, t0, seq);
+    if (n <= 0) return;
+    const int head = blockIdx.y / a.head_tiles, ht = blockIdx.y % a.head_tiles;
+    const int chunk = blockIdx.z;
+    // this lane's row
+    const int r_tok = g / a.rows_heads, r_head = ht * a.rows_heads + g % a.rows_heads;
+    const bool row_ok = r_tok < n && r_head < a.group;
+    const long long most = (long long)a.width * kPage - 1;
+    const int pos = row_ok ? (int)min((long long)a.tok_pos[t0 + r_tok], most) : -1;
+    int last = pos;
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+    const int k0 = chunk * a.chunk;              // n_chunks * chunk may pass what this tile has; the last chunk takes all that is left
+    const int keys = chunk == a.n_chunks - 1 ? last + 1 - k0 : min(last + 1 - k0, a.chunk);
+    if (keys <= 0 && chunk > 0) return;          // chunk 0 writes the rows that attend nothing
+    __syncthreads();                             // barriers are initialised
+
+    // the query rows as the A operand: reg 0, 2: this row's high parts; 1, 3: its low parts
+    uint32_t qa[KS][4];
+    float row_f;
+    {
+        float x[KB];
+        const T* src = static_cast<const T*>(a.q) + (long long)(t0 + (row_ok ? r_tok : 0)) * a.q_stride + (head * a.group + (row_ok ? r_head : 0)) * HD + t * KB;
+        if constexpr (KB >= 8) {
+#pragma unroll
+            for (int i = 0; i < KB; i += 8) load8(src + i, a.wide, x + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < KB; ++i) x[i] = to_float(src[i]);
+        }
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < KB; ++i) top = fmaxf(top, fabsf(x[i]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // f = 2^-e with top in [2^(e-1), 2^e): exponents are kept where f and 1 / f are normal numbers
+        const int e = min(max((int)(__float_as_uint(top) >> 23) - 126, -125), 125);
+        const float f = top > 0.f ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
+        row_f = (top > 0.f ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f) * a.scale * 1.4426950408889634f;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+            if (!row_ok) { x[4 * j] = x[4 * j + 1] = x[4 * j + 2] = x[4 * j + 3] = 0.f; }
+            split2(x[4 * j] * f, x[4 * j + 1] * f, qa[j][0], qa[j][1]);
+            split2(x[4 * j + 2] * f, x[4 * j + 3] * f, qa[j][2], qa[j][3]);
+        }
+    }
+
+    float o[VB][4];
+#pragma unroll
+    for (int j = 0; j < VB; ++j) { o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f; }
+    float m_run = -INFINITY, l_run = 0.f, vr = 0.f, vr_inv = 0.f;
+
+    const int n_units = keys > 0 ? (keys + kA8Unit - 1) / kA8Unit : 0;
+    const int mine = n_units > warp ? (n_units - warp + kA8Warps - 1) / kA8Warps : 0;
+    const int* table = a.table + (size_t)seq * a.width + k0 / kPage;
+    unsigned char* my = smem_raw + (size_t)warp * kA8Stages * STAGE;
+    // pages of 32 of this warp's units at a time, one per lane; -1 stands for a page outside the pool, whose keys do not count
+    auto pages_of = [&](int i0) {
+        const int u = (i0 + lane) * kA8Warps + warp;
+        int p = -1;
+        if (i0 + lane < mine) {
+            p = table[u / (kPage / kA8Unit)];
+            if (p < 0 || p >= a.c.n_pages) { p = -1; if (a.status) atomicExch(a.status, 1); }
+        }
+        return p;
+    };
+    int pid_iss = pages_of(0), pid_use = pid_iss;
+    auto issue = [&](int i) {                    // the warp's unit i, by every lane (one of them copies)
+        if ((i & 31) == 0 && i) pid_iss = pages_of(i);
+        const int page = __shfl_sync(0xffffffffu, pid_iss, i & 31);
+        if (page < 0 || lane != 0) return;
+        const int s = i % kA8Stages, half_page = (i * kA8Warps + warp) % (kPage / kA8Unit);
+        const uint32_t bar = as_smem(&bars[warp][s]), dst = as_smem(my + (size_t)s * STAGE);
+        const long long run = ((long long)page * a.c.H + head) * 2;
+        bar_expect(bar, 2 * RUN + 32);
+        bulk_g2s(dst, a.c.pages + (run * kPage + half_page * kA8Unit) * HD, RUN, bar);
+        bulk_g2s(dst + RUN, a.c.pages + ((run + 1) * kPage + half_page * kA8Unit) * HD, RUN, bar);
+        bulk_g2s(dst + 2 * RUN, a.c.scales + run * kBlksPerPage, 32, bar);
+    };
+    for (int i = 0; i < kA8Stages && i < mine; ++i) issue(i);
+
+    bool ok = true;
+    uint32_t phase = 0;
+    // row of key column g inside a group of 8: pairs of neighbours swap from the third pair on, so that the rows which one
+    // load of V touches are not all even or all odd (rows are 64 bytes at head_dim 64: half the bank conflicts)
+    const int key_of_g = g ^ ((g >> 2) & 1);
+    for (int i = 0; i < mine; ++i) {
+        if ((i & 31) == 0 && i) pid_use = pages_of(i);
+        const int page = __shfl_sync(0xffffffffu, pid_use, i & 31);
+        const int s = i % kA8Stages;
+        if (page >= 0) {
+            ok = bar_wait(as_smem(&bars[warp][s]), (phase >> s) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            phase ^= 1u << s;
+            const unsigned char* sk = my + (size_t)s * STAGE;
+            const unsigned char* sv = sk + RUN;
+            const int unit = i * kA8Warps + warp;
+            const float* scl = reinterpret_cast<const float*>(sk + 2 * RUN) + (unit % (kPage / kA8Unit)) * 2;
+            const int kb = k0 + unit * kA8Unit;                  // first key of the unit
+            float sc[4][4];
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt) {
+                sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+                uint32_t w[KB / 4];
+                const unsigned char* row = sk + (nt * 8 + key_of_g) * HD + t * KB;
+                if constexpr (KB >= 16) {
+#pragma unroll
+                    for (int x = 0; x < KB / 16; ++x) *reinterpret_cast<uint4*>(w + 4 * x) = *reinterpret_cast<const uint4*>(row + 16 * x);
+                } else if constexpr (KB == 8) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(row);
+                else w[0] = *reinterpret_cast<const uint32_t*>(row);
+#pragma unroll
+                for (int j = 0; j < KS; ++j) {
+                    const uint32_t b = w[j] ^ 0x80808080u;
+                    mma16816(sc[nt], qa[j], halves(b, 0x4140), halves(b, 0x4342));
+                }
+            }
+            // scores in units of log2(e), masked by selection: what stands in a masked place is never used
+            float mx = -INFINITY;
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt) {
+                const float f = scl[nt >> 1] * row_f;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int key = kb + nt * 8 + ((2 * t + e) ^ (t >> 1));
+                    sc[nt][e] = key <= pos ? (sc[nt][e] + sc[nt][e + 2]) * f : -INFINITY;
+                    mx = fmaxf(mx, sc[nt][e]);
+                }
+            }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float m_new = fmaxf(m_run, mx);
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;
+            float corr = exp2_fast(m_run - m_use);
+            m_run = m_new;
+            l_run *= corr;
+            const float vs0 = scl[4], vs1 = scl[5];
+            // the second block of a unit may lie behind the last position: its scale is another owner's then and does not count
+            const float vtop = kb + kBlk8 <= last ? fmaxf(vs0, vs1) : vs0;
+            if (vtop > vr) {
+                const float up = pow2_above(fminf(vtop, 1.7e38f));
+                corr *= vr / up;
+                vr = up;
+                vr_inv = 1.f / up;
+            }
+            if (__any_sync(0xffffffffu, corr != 1.f)) {
+#pragma unroll
+                for (int j = 0; j < VB; ++j) { o[j][0] *= corr; o[j][1] *= corr; o[j][2] *= corr; o[j][3] *= corr; }
+            }
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                const float vf = (kk ? vs1 : vs0) * vr_inv;
+                uint32_t pa[4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float p[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int key = kb + (2 * kk + h) * 8 + ((2 * t + e) ^ (t >> 1));
+                        p[e] = exp2_fast(sc[2 * kk + h][e] - m_use);
+                        l_run += p[e];
+                        p[e] = key <= pos ? p[e] * vf : 0.f;
+                    }
+                    split2(p[0], p[1], pa[2 * h], pa[2 * h + 1]);
+                }
+                // V rows of keys (2t, 2t + 1) and (2t + 8, 2t + 9) of this block, as permuted above
+                const unsigned char* row = sv + (kk * kBlk8) * HD + g * VB;
+                const int e0 = (2 * t) ^ (t >> 1), e1 = (2 * t + 1) ^ (t >> 1);
+                if constexpr (VB >= 4) {
+                    constexpr int NW = VB / 4;
+                    uint32_t v[4][NW];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const unsigned char* src = row + ((x & 1 ? e1 : e0) + (x >> 1) * 8) * HD;
+                        if constexpr (NW == 4) *reinterpret_cast<uint4*>(v[x]) = *reinterpret_cast<const uint4*>(src);
+                        else if constexpr (NW == 2) *reinterpret_cast<uint2*>(v[x]) = *reinterpret_cast<const uint2*>(src);
+                        else v[x][0] = *reinterpret_cast<const uint32_t*>(src);
+                    }
+#pragma unroll
+                    for (int w = 0; w < NW; ++w) {
+                        const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140) ^ 0x80808080u, a1 = __byte_perm(v[0][w], v[1][w], 0x7362) ^ 0x80808080u;
+                        const uint32_t b0 = __byte_perm(v[2][w], v[3][w], 0x5140) ^ 0x80808080u, b1 = __byte_perm(v[2][w], v[3][w], 0x7362) ^ 0x80808080u;
+                        mma16816(o[4 * w], pa, halves(a0, 0x4140), halves(b0, 0x4140));
+                        mma16816(o[4 * w + 1], pa, halves(a0, 0x4342), halves(b0, 0x4342));
+                        mma16816(o[4 * w + 2], pa, halves(a1, 0x4140), halves(b1, 0x4140));
+                        mma16816(o[4 * w + 3], pa, halves(a1, 0x4342), halves(b1, 0x4342));
+                    }
+                } else {                                         // head_dim 16: two bytes of each row
+                    uint32_t v[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) v[x] = *reinterpret_cast<const uint16_t*>(row + ((x & 1 ? e1 : e0) + (x >> 1) * 8) * HD);
+                    const uint32_t a0 = __byte_perm(v[0], v[1], 0x5140) ^ 0x80808080u, b0 = __byte_perm(v[2], v[3], 0x5140) ^ 0x80808080u;
+                    mma16816(o[0], pa, halves(a0, 0x4140), halves(b0, 0x4140));
+                    mma16816(o[1], pa, halves(a0, 0x4342), halves(b0, 0x4342));
+                }
+            }
+            __syncwarp();                                        // every lane is done with stage s
+        }
+        if (i + kA8Stages < mine) issue(i + kA8Stages);
+    }
+    if (!ok) { s_ok = 0; if (a.status) atomicExch(a.status, 5); }
+    l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
+    l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
+    if (t == 0) { s_m[warp][g] = m_run; s_l[warp][g] = l_run; }
+    __syncthreads();                                             // every warp is done with its stages: their memory is used again
+    if (!s_ok) {                                                 // let copies in flight land before shared memory is released
+        for (int i = 0; i < 32; ++i) __nanosleep(16384);
+        return;
+    }
+    constexpr int OS = HD + 4;                                   // floats per row: rows start in different banks
+    static_assert((size_t)kA8Warps * kA8Rows * OS * 4 <= attn8_smem<HD>(), "the joined states fit the stages");
+    float* so = reinterpret_cast<float*>(smem_raw);
+#pragma unroll
+    for (int j = 0; j < VB; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)                              // column 2t + e of column tile j is dim (2t + e) VB + j
+            so[(warp * kA8Rows + g) * OS + (2 * t + e) * VB + j] = (o[j][e] + o[j][e + 2]) * vr;
+    __syncthreads();
+    // eight dims per thread at a time: the four states joined in the order of the warps
+    for (int x = tid; x < kA8Rows * HD / 8; x += kA8Threads) {
+        const int r = x / (HD / 8), d = (x % (HD / 8)) * 8;
+        const int rt = r / a.rows_heads, rh = ht * a.rows_heads + r % a.rows_heads;
+        if (rt >= n || rh >= a.group) continue;
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kA8Warps; ++w) m = fmaxf(m, s_m[w][r]);
+        float l = 0.f, f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kA8Warps; ++w) {
+            // a state whose scores are all NaN has no maximum, but its sum says so
+            const float wt = s_m[w][r] == -INFINITY ? (s_l[w][r] == 0.f ? 0.f : 1.f) : exp2_fast(s_m[w][r] - m);
+            if (wt == 0.f && s_l[w][r] == 0.f) continue;
+            l += wt * s_l[w][r];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] += wt * so[(w * kA8Rows + r) * OS + d + k];
+        }
+        const long long tok = t0 + rt;
+        const int qh = head * a.group + rh;
+        const int own_chunks = attn8_chunks(a, last);
+        if (own_chunks <= 1) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] *= inv;
+            store8(static_cast<T*>(a.out) + tok * a.out_stride + qh * HD + d, a.wide, f);
+        } else {
+            const long long pi = (tok * a.n_heads + qh) * a.n_chunks + chunk;
+            store8(a.part + pi * HD + d, true, f);
+            if (d == 0) { a.part_ml[pi * 2] = m; a.part_ml[pi * 2 + 1] = l; }
+        }
+    }
+}
+
+// Joins the chunks of each (token, head), in their order: one warp each.  A row whose tile had one chunk is written already;
+// a tile's chunks are those of its last row, so a row may have chunks in which it attends nothing (m = -inf, l = 0).
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) k_attn_kv8_join(const Attn8Args a) {
+    pdl_wait();
+    const long long x = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (x >= (long long)a.n_tok * a.n_heads) return;
+    const int tok = (int)(x / a.n_heads), qh = (int)(x % a.n_heads);
+    const int seq = a.tok_seq[tok];
+    if (seq < 0 || seq >= a.n_seq) return;
+    int last = tok;                                              // the tile's last token
+    if (a.cu_tok) {
+        const int first = a.cu_tok[seq], end = min(a.cu_tok[seq + 1], a.n_tok);
+        if (tok < first || tok >= end) return;                   // the lists contradict one another: no tile had this row
+        last = min(first + (tok - first) / a.rows_toks * a.rows_toks + a.rows_toks, end) - 1;
+    }
+    int lp = -1;
+    for (int i = a.cu_tok ? a.cu_tok[seq] + (tok - a.cu_tok[seq]) / a.rows_toks * a.rows_toks : tok; i <= last; ++i) lp = max(lp, a.tok_pos[i]);
+    lp = (int)min((long long)lp, (long long)a.width * kPage - 1);
+    const int chunks = attn8_chunks(a, lp);
+    if (chunks <= 1) return;
+    const long long p0 = x * a.n_chunks;
+    float m = -INFINITY;
+    for (int c = lane; c < chunks; c += 32) m = fmaxf(m, a.part_ml[(p0 + c) * 2]);
+    m = warp_max(m);
+    constexpr int DL = HD >= 32 ? HD / 32 : 1;
+    float l = 0.f, f[DL];
+#pragma unroll
+    for (int k = 0; k < DL; ++k) f[k] = 0.f;
+    for (int c = 0; c < chunks; ++c) {
+        const float mc = a.part_ml[(p0 + c) * 2], lc = a.part_ml[(p0 + c) * 2 + 1];
+        const float wt = mc == -INFINITY ? (lc == 0.f ? 0.f : 1.f) : exp2_fast(mc - m);
+        if (wt == 0.f && lc == 0.f) continue;
+        l += wt * lc;
+        if (lane * DL < HD)
+#pragma unroll
+            for (int k = 0; k < DL; ++k) f[k] += wt * a.part[(p0 + c) * HD + lane * DL + k];
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (lane * DL < HD) {
+        T* dst = static_cast<T*>(a.out) + (long long)tok * a.out_stride + qh * HD + lane * DL;
+#pragma unroll
+        for (int k = 0; k < DL; ++k) dst[k] = from_float<T>(f[k] * inv);
+    }
+}
+
+}  // namespace sllm

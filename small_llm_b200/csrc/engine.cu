@@ -23,6 +23,7 @@
 #include <vector>
 
 #include "../../include/sllm.h"
+#include "abi.cuh"
 #include "attn_decode.cuh"
 #include "attn_prefill.cuh"
 #include "attn_prefill_tc.cuh"
@@ -40,6 +41,15 @@ using namespace sllm;
 namespace {
 
 thread_local std::string g_create_error;
+
+}  // namespace
+
+int sllm::fail_text(int code, const char* msg) noexcept {
+    try { g_create_error = msg; } catch (...) {}
+    return code;
+}
+
+namespace {
 
 struct ParamSlot {
     std::string name;
