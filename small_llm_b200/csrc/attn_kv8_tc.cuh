@@ -1,0 +1,400 @@
+// Attention over the 8-bit paged cache (kv8.cuh) for prompts: bf16 rows, head_dim 64 or 128, on the 5th-generation tensor cores.
+//
+// One block takes one kv head and two tiles of 128 query rows (tokens x heads of the group) that follow on one another, so
+// that a key is widened once for 256 rows.  Per step of 128 keys (two pages):
+//   widening warps   int8 K and V from global memory (a step ahead, in registers) -> fp16 in shared memory, 128-byte swizzle
+//   MMA warp         S_t = Q_t K^T, 128 x 128 x hd;  O_t += P_t V, 128 x hd x 128, accumulated in tensor memory   (t = 0, 1)
+//   softmax t        thread = query row = TMEM lane: w = exp2(...) as fp16 over S_t's own columns, where the next product reads it
+// While one tile's softmax runs, the tensor cores work on the other's products.
+//
+// The integers are multiplied as they are (exact in fp16), scales act outside the products and cost nothing per element: with
+// c = scale log2(e) ks(block) and v = vs(block) / vr the weight is  w = p v = exp2(S c + (log2 v - m)),  one fma and one ex2, and
+// the softmax denominator sums w / v block by block.  vr, a power of two no smaller than any vs so far, keeps w in fp16's range.
+// w is rounded to fp16 (2^-11 of a weight; the output is rounded to bf16, 2^-8) and q, bf16 divided by a power of two, is
+// exact in fp16 down to 2^-16 of the row's largest value.  m is not the running maximum itself but follows it when it is
+// passed by more than 8 (a factor of 256, which fp16 and the fp32 sums take): O in tensor memory is then rescaled, which is rare.
+//
+// Bound by the exponentials (16 a clock and SM: 1024 clocks per 128 x 128 tile) and, at head_dim 128, equally by the products.
+// Every wait is bounded; on expiry the block sets *status, frees its tensor memory and returns.
+#pragma once
+#include "attn_kv8.cuh"
+#include "tc_ptx.cuh"
+
+namespace sllm {
+
+constexpr int kT8Rows = 128;                     // query rows of a tile
+constexpr int kT8Keys = 128;                     // keys of a step
+constexpr int kT8SoftWarps = 8, kT8WideWarps = 4;
+constexpr int kT8Threads = (kT8SoftWarps + kT8WideWarps + 1) * 32;
+constexpr int kT8Blks = kT8Keys / kBlk8;         // scale blocks of a step
+constexpr int kT8Ring = 4;                       // steps whose scales are held
+constexpr float kT8Slack = 8.f;                  // log2 units that scores may pass m by
+
+template <int HD> __host__ __device__ constexpr size_t attn8_tc_smem() {
+    return 1024 + 2 * (size_t)kT8Rows * HD * 2 + 4 * (size_t)kT8Keys * HD * 2 + kT8Ring * (kT8Blks + 1) * 16 + 256;
+}
+
+__device__ __forceinline__ bool wait8(uint32_t bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, kWaitLimitNs); }
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+                 ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int HD>
+__global__ void __launch_bounds__(kT8Threads, 1) k_attn_kv8_tc(const Attn8Args a) {
+    constexpr int HALVES = HD / 64;                           // 128-byte column blocks of a row
+    constexpr uint32_t HALF = kT8Keys * 128;                  // bytes of one of them (query rows and keys are both 128)
+    constexpr uint32_t TILE = HALVES * HALF;
+    constexpr int CPR = HD / 16;                              // 16-byte chunks of int8 per cache row
+    constexpr int RPP = kT8WideWarps * 32 / CPR;              // rows per pass of the widening threads
+    constexpr int PASSES = kT8Keys / RPP;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* sQ = smem;                                       // [2][TILE]
+    uint8_t* sK = sQ + 2 * TILE;                              // [2 stages][TILE]
+    uint8_t* sV = sK + 2 * TILE;
+    float4* s_blk = reinterpret_cast<float4*>(sV + 2 * TILE); // [ring][blocks]: c, log2 v, 1 / v, 0 or -inf (blocks that do not count)
+    float4* s_vr = s_blk + kT8Ring * kT8Blks;                 // [ring]: vr
+    uint64_t* bars = reinterpret_cast<uint64_t*>(s_vr + kT8Ring);
+    enum { K_FULL = 0, V_FULL = 2, K_FREE = 4, V_FREE = 6, S_READY = 8, P_READY = 10, SC_FULL = 12, O_DONE = 16, N_BARS = 17 };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
+    __shared__ int s_last[kT8SoftWarps];
+    const uint32_t bar0 = smem_u32(bars);
+    auto B = [&](int i) { return bar0 + 8u * (uint32_t)i; };
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_launch_dependents();
+    pdl_wait();
+    int t0, seq;
+    const int n = attn8_tile(a, gridDim.x - 1 - blockIdx.x, t0, seq);      // late tiles, which have the most keys, first
+    if (n <= 0) return;
+    const int head = blockIdx.y, group = a.group, toks = a.rows_toks >> 1; // tokens of one tile
+    const int most = (int)min((long long)a.width * kPage, 0x7fffff00ll) - 1;
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(B(K_FULL + i), kT8WideWarps); mbar_init(B(V_FULL + i), kT8WideWarps);
+            mbar_init(B(K_FREE + i), 1); mbar_init(B(V_FREE + i), 1);
+            mbar_init(B(S_READY + i), 1); mbar_init(B(P_READY + i), 4);
+        }
+        for (int i = 0; i < kT8Ring; ++i) mbar_init(B(SC_FULL + i), 1);
+        mbar_init(B(O_DONE), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kT8SoftWarps + kT8WideWarps) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+
+    // the softmax threads' rows, and Q as fp16, K-major with the 128-byte swizzle; rows of no token are zero
+    const int tile = warp >> 2, r = tid & 127;                // of the softmax warps
+    int pos = 0, row_tok = -1, row_head = 0;
+    float row_f = 0.f;
+    if (warp < kT8SoftWarps) {
+        const int rt = tile * toks + r / group;
+        const bool valid = r / group < toks && rt < n;
+        if (valid) { row_tok = t0 + rt; row_head = head * group + r % group; }
+        pos = valid ? min(a.tok_pos[row_tok], most) : -1;
+        const int last_w = __reduce_max_sync(0xffffffffu, pos);
+        if (lane == 0) s_last[warp] = last_w;
+        uint4 raw[HD / 8];
+        const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + (valid ? (long long)row_tok * a.q_stride + row_head * HD : 0);
+        unsigned top = 0;
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+            raw[c] = make_uint4(0u, 0u, 0u, 0u);
+            if (valid) {
+                if (a.wide) raw[c] = *reinterpret_cast<const uint4*>(src + 8 * c);
+                else {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        w[j] = (uint32_t)__bfloat16_as_ushort(src[8 * c + 2 * j]) | (uint32_t)__bfloat16_as_ushort(src[8 * c + 2 * j + 1]) << 16;
+                    raw[c] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[c]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = max(top, max((w[j] & 0x7fffu) << 16, w[j] & 0x7fff0000u));
+        }
+        // f = 2^-e with the largest value in [2^(e-1), 2^e), as in the general kernel
+        const int e = min(max((int)(top >> 23) - 126, -125), 125);
+        const float f = top ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
+        row_f = top ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
+        const float fs = a.scale < 0.f ? -f : f;              // block factors are positive: a maximum may be taken before them
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+            float x[8];
+            unpack16<__nv_bfloat16>(raw[c], x);
+            *reinterpret_cast<uint4*>(sQ + tile * TILE + (c >> 3) * HALF + sw128(r, c & 7)) =
+                make_uint4(pack_half(x[0] * fs, x[1] * fs), pack_half(x[2] * fs, x[3] * fs), pack_half(x[4] * fs, x[5] * fs), pack_half(x[6] * fs, x[7] * fs));
+        }
+        fence_async_smem();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int last0 = max(max(s_last[0], s_last[1]), max(s_last[2], s_last[3]));
+    const int last1 = max(max(s_last[4], s_last[5]), max(s_last[6], s_last[7]));
+    const int last = max(last0, last1);
+    const int n0 = (last0 + kT8Keys) / kT8Keys, n1 = (last1 + kT8Keys) / kT8Keys, steps = max(n0, n1);     // 0 where nothing is attended
+    bool ok = true;
+
+    if (warp == kT8SoftWarps + kT8WideWarps) {
+        // ---- MMA ----
+        if (lane == 0) {
+            const uint32_t id_s = (1u << 4) | ((uint32_t)(kT8Keys >> 3) << 17) | ((uint32_t)(kT8Rows >> 4) << 24);     // fp16 x fp16 -> fp32
+            const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(kT8Rows >> 4) << 24);   // V: MN-major
+            auto issue_s = [&](int i, int t) {
+                const uint32_t q = smem_u32(sQ) + t * TILE, k = smem_u32(sK) + (i & 1) * TILE;
+#pragma unroll
+                for (int j = 0; j < HD / 16; ++j) {
+                    const uint32_t at = (j >> 2) * HALF + (j & 3) * 32;
+                    tc_mma_bf16(tmem + (uint32_t)(t * kT8Keys), tc_smem_desc(q + at), tc_smem_desc(k + at), id_s, j != 0);
+                }
+                tc_commit(B(S_READY + t));
+            };
+            auto issue_o = [&](int i, int t) {
+                const uint32_t v = smem_u32(sV) + (i & 1) * TILE;
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+                    for (int j = 0; j < kT8Keys / 16; ++j)
+                        tc_mma_f16_ts(tmem + 2 * kT8Keys + t * HD + h * 64, tmem + (uint32_t)(t * kT8Keys + j * 8), tc_smem_desc(v + h * HALF + j * 2048), id_o, i > 0 || j > 0);
+            };
+            if (steps > 0) {
+                ok = wait8(B(K_FULL), 0);
+                tc_fence_after();
+                if (ok && n0 > 0) issue_s(0, 0);
+                if (ok && n1 > 0) issue_s(0, 1);
+                if (ok) tc_commit(B(K_FREE));
+            }
+            for (int i = 0; i < steps && ok; ++i) {
+                const int s = i & 1;
+                ok = wait8(B(V_FULL + s), (i >> 1) & 1);
+                for (int t = 0; t < 2 && ok; ++t) {
+                    const int nt = t ? n1 : n0;
+                    if (i < nt) {
+                        ok = wait8(B(P_READY + t), i & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        issue_o(i, t);
+                    }
+                    if (i + 1 < nt) {
+                        ok = wait8(B(K_FULL + (s ^ 1)), ((i + 1) >> 1) & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        issue_s(i + 1, t);
+                    }
+                }
+                if (!ok) break;
+                tc_commit(B(V_FREE + s));
+                if (i + 1 < steps) tc_commit(B(K_FREE + (s ^ 1)));
+            }
+            if (ok && steps > 0) tc_commit(B(O_DONE));
+        }
+    } else if (warp >= kT8SoftWarps) {
+        // ---- widening: int8 rows -> fp16 tiles, and the blocks' factors ----
+        const int w = tid - kT8SoftWarps * 32, c = w % CPR, row0 = w / CPR;
+        const int* table = a.table + (size_t)seq * a.width;
+        const int8_t* pool = a.c.pages;
+        auto page_of = [&](int i, int half) -> int {          // -1: behind the last position, -2: outside the pool
+            const int p = 2 * i + half;
+            if ((long long)p * kPage > last) return -1;
+            const int id = table[p];
+            if (id < 0 || id >= a.c.n_pages) { if (a.status && w == 0) atomicExch(a.status, 1); return -2; }
+            return id;
+        };
+        auto fetch = [&](int p0, int p1, int which, uint4 (&x)[PASSES]) {
+#pragma unroll
+            for (int j = 0; j < PASSES; ++j) {
+                const int row = row0 + j * RPP, id = j < PASSES / 2 ? p0 : p1;
+                x[j] = make_uint4(0u, 0u, 0u, 0u);
+                if (id >= 0)
+                    x[j] = *reinterpret_cast<const uint4*>(pool + ((((long long)id * a.c.H + head) * 2 + which) * kPage + (row & (kPage - 1))) * HD + c * 16);
+            }
+        };
+        auto widen = [&](uint8_t* dst, const uint4 (&x)[PASSES]) {
+            const int swap = HALVES == 2 ? (c >> 2) & 1 : 0;   // the two column blocks store their halves of a chunk in opposite order: no bank conflicts
+#pragma unroll
+            for (int j = 0; j < PASSES; ++j) {
+                const int row = row0 + j * RPP;
+                const uint32_t u[4] = {x[j].x ^ 0x80808080u, x[j].y ^ 0x80808080u, x[j].z ^ 0x80808080u, x[j].w ^ 0x80808080u};
+                const uint4 lo = make_uint4(halves(u[0], 0x4140), halves(u[0], 0x4342), halves(u[1], 0x4140), halves(u[1], 0x4342));
+                const uint4 hi = make_uint4(halves(u[2], 0x4140), halves(u[2], 0x4342), halves(u[3], 0x4140), halves(u[3], 0x4342));
+                uint8_t* base = dst + (c >> 2) * HALF;
+                const int ch = (2 * c) & 7;
+                *reinterpret_cast<uint4*>(base + sw128(row, ch + swap)) = swap ? hi : lo;
+                *reinterpret_cast<uint4*>(base + sw128(row, ch + 1 - swap)) = swap ? lo : hi;
+            }
+            fence_async_smem();
+            __syncwarp();
+        };
+        uint4 xk[PASSES], xv[PASSES];
+        int p0 = -1, p1 = -1;
+        float vr = 0.f;
+        if (steps > 0) { p0 = page_of(0, 0); p1 = page_of(0, 1); fetch(p0, p1, 0, xk); }
+        for (int i = 0; i < steps && ok; ++i) {
+            const int s = i & 1;
+            // scales of this step's blocks: lane b of the first warp takes block b
+            float ks = 0.f, vs = 0.f;
+            bool counts = false;
+            if (w < kT8Blks) {
+                const int id = w < kBlksPerPage ? p0 : p1;
+                counts = id >= 0 && (long long)i * kT8Keys + w * kBlk8 <= last;
+                if (counts) {
+                    const float* sc = a.c.scales + ((long long)id * a.c.H + head) * 2 * kBlksPerPage + (w % kBlksPerPage);
+                    ks = sc[0]; vs = sc[kBlksPerPage];
+                }
+            }
+            fetch(p0, p1, 1, xv);
+            int q0 = -1, q1 = -1;
+            if (i + 1 < steps) { q0 = page_of(i + 1, 0); q1 = page_of(i + 1, 1); }
+            if (i >= 2) ok = wait8(B(K_FREE + s), ((i >> 1) - 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (w < 32) {
+                // K_FREE of step i - 2 means that the softmax is done with step i - 3: its place in the ring may be written
+                float top = counts && vs == vs ? vs : 0.f;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                if (top > vr) vr = pow2_above(fminf(top, 1.7e38f));
+                if (w < kT8Blks) {
+                    const float v0 = vr > 0.f ? vs / vr : (vs == 0.f ? 1.f : vs);
+                    const float v = v0 != v0 ? v0 : fmaxf(v0, 8.67361738e-19f);          // 2^-60: fp16 takes such a weight for 0, the sum does not
+                    s_blk[(i % kT8Ring) * kT8Blks + w] = counts ? make_float4(ks * fabsf(a.scale) * 1.4426950408889634f, log2f(v), 1.f / v, 0.f)
+                                                                : make_float4(0.f, -INFINITY, 0.f, -INFINITY);
+                }
+                if (w == 0) s_vr[i % kT8Ring].x = vr;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(B(SC_FULL + i % kT8Ring));
+            }
+            widen(sK + s * TILE, xk);
+            if (lane == 0) mbar_arrive(B(K_FULL + s));
+            p0 = q0; p1 = q1;
+            if (i + 1 < steps) fetch(p0, p1, 0, xk);
+            if (i >= 2) ok = wait8(B(V_FREE + s), ((i >> 1) - 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            widen(sV + s * TILE, xv);
+            if (lane == 0) mbar_arrive(B(V_FULL + s));
+        }
+    } else {
+        // ---- softmax: thread = query row = TMEM lane ----
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t s_at = lanes + tile * kT8Keys, o_at = lanes + 2 * kT8Keys + tile * HD;
+        const int my_steps = tile ? n1 : n0;
+        const int open = row_tok >= 0 ? pos : 0x7fffffff;      // rows of no token: q = 0, whatever they come to is not written
+        const int all_see = __reduce_min_sync(0xffffffffu, open);
+        float m = -INFINITY, l = 0.f, vr = 0.f;
+        for (int i = 0; i < my_steps && ok; ++i) {
+            ok = wait8(B(SC_FULL + i % kT8Ring), (i / kT8Ring) & 1) && wait8(B(S_READY + tile), i & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const float4* blk = s_blk + (i % kT8Ring) * kT8Blks;
+            const int kb = i * kT8Keys;
+            const bool masked = kb + kT8Keys - 1 > all_see;    // the same for the whole warp
+            uint32_t sv[32];
+            float mx = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < kT8Keys / 32; ++h) {
+                tc_ld32(s_at + h * 32, sv);
+                if (masked) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (kb + h * 32 + j > open) sv[j] = 0xff800000u;
+                }
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    float t4[4] = {__uint_as_float(sv[b * 16]), __uint_as_float(sv[b * 16 + 1]), __uint_as_float(sv[b * 16 + 2]), __uint_as_float(sv[b * 16 + 3])};
+#pragma unroll
+                    for (int j = 4; j < 16; ++j) t4[j & 3] = fmaxf(t4[j & 3], __uint_as_float(sv[b * 16 + j]));
+                    const float4 f = blk[h * 2 + b];
+                    mx = fmaxf(mx, fmaf(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])), f.x * row_f, f.w));
+                }
+            }
+            const float vr_now = s_vr[i % kT8Ring].x;
+            const bool moves = mx > m + kT8Slack || (m == -INFINITY && mx > m);
+            if (__any_sync(0xffffffffu, moves || vr_now != vr)) {
+                const float m_new = moves ? mx : m;
+                const float corr = m == -INFINITY ? 0.f : exp2_fast(m - m_new);
+                l *= corr;
+                if (i > 0) {                                   // every product into O so far is done: S of this step came after them
+                    const float f = corr * (vr_now > 0.f ? vr / vr_now : 1.f);
+#pragma unroll
+                    for (int h = 0; h < HD / 16; ++h) {
+                        tc_ld16(o_at + h * 16, sv);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) sv[j] = __float_as_uint(__uint_as_float(sv[j]) * f);
+                        tc_st16(o_at + h * 16, sv);
+                    }
+                }
+                m = m_new;
+                vr = vr_now;
+            }
+            const float m_use = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int h = 0; h < kT8Keys / 32; ++h) {
+                tc_ld32(s_at + h * 32, sv);
+                uint32_t pk[16];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const float4 f = blk[h * 2 + b];
+                    const float c = f.x * row_f, d = f.y - m_use;
+                    float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        float w0 = exp2_fast(fmaf(__uint_as_float(sv[b * 16 + j]), c, d));
+                        float w1 = exp2_fast(fmaf(__uint_as_float(sv[b * 16 + j + 1]), c, d));
+                        if (masked) {
+                            if (kb + h * 32 + b * 16 + j > open) w0 = 0.f;
+                            if (kb + h * 32 + b * 16 + j + 1 > open) w1 = 0.f;
+                        }
+                        sum0 += w0; sum1 += w1;
+                        pk[b * 8 + j / 2] = pack_half(w0, w1);
+                    }
+                    l = fmaf(sum0 + sum1, f.z, l);
+                }
+                tc_st16(s_at + h * 16, pk);                    // over columns of S that this thread has read
+            }
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(B(P_READY + tile));
+        }
+        if (steps > 0 && ok) ok = wait8(B(O_DONE), 0);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+        if (ok) {
+            const float inv = l == 0.f ? 0.f : vr / l;
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (row_tok >= 0 ? (long long)row_tok * a.out_stride + row_head * HD : 0);
+#pragma unroll
+            for (int h = 0; h < HD / 16; ++h) {
+                uint32_t o[16];
+                if (my_steps > 0) tc_ld16(o_at + h * 16, o);
+                float x[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] = l == 0.f || my_steps == 0 ? 0.f : __uint_as_float(o[j]) * inv;
+                if (row_tok >= 0) { store8(dst + h * 16, a.wide, x); store8(dst + h * 16 + 8, a.wide, x + 8); }
+            }
+        }
+    }
+    if (!ok && a.status) atomicExch(a.status, 5);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kT8SoftWarps + kT8WideWarps) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+}  // namespace sllm

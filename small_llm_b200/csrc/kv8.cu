@@ -9,6 +9,7 @@
 #include "../../include/sllm.h"
 #include "abi.cuh"
 #include "attn_kv8.cuh"
+#include "attn_kv8_tc.cuh"
 #include "kv8.cuh"
 
 using namespace sllm;
@@ -128,7 +129,7 @@ int check_rows(const char* what, const sllm_kv8_layer* c, const sllm_kv8_rows* r
 }
 
 // ---- attention: which form, how the work is cut -----------------------------------------------------------------
-struct Plan { Attn8Args a; unsigned tiles; };
+struct Plan { Attn8Args a; unsigned tiles; bool tc; };
 
 Plan plan_attn(const sllm_kv8_layer* c, const sllm_kv8_attn* s, int sms) {
     Plan p{};
@@ -147,6 +148,15 @@ Plan plan_attn(const sllm_kv8_layer* c, const sllm_kv8_attn* s, int sms) {
     a.wide = aligned(s->q, 16) && aligned(s->out, 16) && (s->q_stride * w) % 16 == 0 && (s->out_stride * w) % 16 == 0;
     a.scale = s->scale != 0.f ? s->scale : 1.0f / std::sqrt((float)c->head_dim);
     a.status = s->status;
+    // Runs of many rows take the tensor-core form.
+    const long long run = s->max_new ? s->max_new : s->n_tok;
+    p.tc = a.cu_tok && s->dtype == SLLM_ROWS_BF16 && c->head_dim >= 64 && a.group <= kT8Rows && run * a.group >= 64;
+    if (p.tc) {
+        a.rows_toks = 2 * (kT8Rows / a.group);
+        p.tiles = s->n_tok / a.rows_toks + s->n_seq;
+        a.n_chunks = 1;
+        return p;
+    }
     // chunks of the keys: until there are two rounds of blocks, and none shorter than one unit per warp
     const long long most = (long long)s->table_width * kPage, len = s->max_len ? std::min<long long>(s->max_len, most) : most;
     const long long base = (long long)p.tiles * c->kv_heads * a.head_tiles;
@@ -194,6 +204,13 @@ int attn_hd(const Plan& p, int dev, void* stream) {
     if (a.n_chunks == 1) return SLLM_OK;
     const long long pairs = (long long)a.n_tok * a.n_heads;
     return launch(what, k_attn_kv8_join<T, HD>, dim3((unsigned)((pairs + 3) / 4)), 128, 0, stream, a);
+}
+template <int HD>
+int attn_tc(const Plan& p, int dev, void* stream) {
+    static std::atomic<uint64_t> done{0};
+    const char* what = "sllm_k_attn_kv8";
+    if (int rc = opt_in(what, k_attn_kv8_tc<HD>, attn8_tc_smem<HD>(), dev, done)) return rc;
+    return launch(what, k_attn_kv8_tc<HD>, dim3(p.tiles, p.a.c.H), kT8Threads, attn8_tc_smem<HD>(), stream, p.a);
 }
 template <typename T>
 int attn_t(const Plan& p, uint32_t hd, int dev, void* stream) {
@@ -279,6 +296,7 @@ int sllm_k_attn_kv8(const sllm_kv8_layer* c, const sllm_kv8_attn* s, void* works
         p.a.part = static_cast<float*>(workspace);
         p.a.part_ml = p.a.part + (size_t)p.a.n_tok * p.a.n_heads * p.a.n_chunks * c->head_dim;
     }
+    if (p.tc) return c->head_dim == 64 ? attn_tc<64>(p, dev, stream) : attn_tc<128>(p, dev, stream);
     return s->dtype == SLLM_ROWS_F32 ? attn_t<float>(p, c->head_dim, dev, stream) : attn_t<__nv_bfloat16>(p, c->head_dim, dev, stream);
 }
 

@@ -4,7 +4,10 @@ Tolerances.  Integers, scales and lists are compared exactly.  Attention in fp32
 units of log2 carries a relative error of about 4 half steps (the split query and three products) plus the accumulation of
 head_dim terms, and as an exponent turns it into a relative error of its weight; weights add the exponential's 2 units in the
 last place and the split's 2^-22; sums of n terms add n half steps at most.  The sum is over weights that add up to one, so all of
-it is relative to the largest value.  bf16 adds half a step of its own, eps / 2 = 2^-8 of the value.
+it is relative to the largest value.  bf16 adds half a step of its own, eps / 2 = 2^-8 of the value; and its form for prompts rounds
+each weight to fp16 before the product with V: half a step, eps / 2 = 2^-11 of the weight, where the denominator keeps the
+unrounded one.  sum_j 2^-11 p_j |v_j| / sum_j p_j is at most 2^-11 of the largest value.  (Weights below fp16's normal range are
+off by 2^-25 absolutely, with the largest at 1 or more: the sums' term covers that.)
 """
 import itertools
 import math
@@ -310,7 +313,7 @@ def _tol(want, top, smax, keys, d, dtype):
     u = 2.0 ** -24
     weight = smax * 1.4427 * (8 + d) * u + 2 * 2.0 ** -22 + 2.0 ** -22      # scores (exponent), exponential, split
     tol = top * (2 * weight + 2 * keys * u)                                  # numerator and denominator
-    return tol + (want.abs() * 2.0 ** -8 if dtype == torch.bfloat16 else want.abs() * u)
+    return tol + (want.abs() * 2.0 ** -8 + top * 2.0 ** -11 if dtype == torch.bfloat16 else want.abs() * u)
 
 
 def check_attention(args, dtype, scale=None, keys=None, **kw):
@@ -365,6 +368,52 @@ def test_long_rows_in_chunks(h, grp, d, dtype):
     check_attention(a, dtype, max_new=1, max_len=9001)
     b = setup_attention([5000, 130], [3, 5], h, grp, d, dtype, seed=4)
     check_attention(b, dtype, max_new=5, max_len=5003, cu_tok=b[6])
+
+
+@pytest.mark.parametrize("h,grp,d", [(1, 1, 64), (2, 4, 128), (1, 8, 64), (1, 5, 128), (1, 20, 64), (2, 1, 128)])
+def test_long_prompts(h, grp, d):
+    """Several tiles of query rows and steps of keys: from position 0, behind histories, ends on and off every border."""
+    a = setup_attention([0, 640, 1, 127], [300, 257, 128, 70], h, grp, d, torch.bfloat16, seed=d + grp)
+    check_attention(a, torch.bfloat16, max_new=300, max_len=897, cu_tok=a[6])
+    b = setup_attention([0, 3000], [64, 90], h, grp, d, torch.bfloat16, seed=d - grp, sharp=6.0)
+    check_attention(b, torch.bfloat16, max_new=90, max_len=3090, cu_tok=b[6], scale=-0.2)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("order", [1, -1])
+def test_prompts_with_scales_of_many_magnitudes(d, order):
+    """Scales that grow, or fall, by 2^24 along the sequence, zeros among them: the running references move many times."""
+    q, pages, scales, table, seq, pos, cu = setup_attention([100, 0], [200, 260], 2, 2, d, torch.bfloat16, seed=77)
+    for i in range(2):
+        for p in range(5):
+            f = 2.0 ** (order * (6 * p - 12))
+            scales[int(table[i, p])] = torch.rand(2, 2, 4, device="cuda", generator=gen(p)) * 0.02 * torch.tensor([1.0, f], device="cuda")[:, None]
+    scales[int(table[0, 1]), 0] = 0.0
+    scales[int(table[1, 0]), 1, 1] = 0.0
+    for rows in (torch.bfloat16, torch.float32):
+        check_attention((q.to(rows), pages, scales, table, seq, pos, cu), rows, max_new=260, max_len=300, cu_tok=cu)
+        check_attention((q.to(rows), pages, scales, table, seq, pos, cu), rows, max_new=1, max_len=300)
+
+
+def test_prompts_with_bad_pages_and_values_that_are_not_finite():
+    q, pages, scales, table, seq, pos, cu = setup_attention([0, 0], [260, 150], 2, 2, 64, torch.bfloat16, seed=78)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    kw = dict(max_new=260, max_len=260)
+    clean = kv8.attention(q, pages, scales, table, seq, pos, cu, **kw)
+    scales[int(table[0, 3]), 1, 0, 1] = math.nan                             # keys 208 .. 223, kv head 1
+    q2 = q.clone()
+    q2[300, 2, 7] = math.nan
+    q2[301, 0, 7] = math.inf
+    got = kv8.attention(q2, pages, scales, table, seq, pos, cu, status=status, **kw)
+    want = torch.zeros(410, 4, dtype=torch.bool)
+    want[208:260, 2:] = True
+    want[300, 2] = want[301, 0] = True
+    assert torch.equal(torch.isnan(got).any(-1).cpu(), want) and torch.equal(got[~want.cuda()], clean[~want.cuda()]) and int(status) == 0
+    scales[int(table[0, 3]), 1, 0, 1] = 0.01
+    table[0, 1], table[1, 0] = -1, 1 << 30
+    pos[5], pos[399] = -1, -7
+    got = check_attention((q, pages, scales, table, seq, pos, cu), torch.bfloat16, cu_tok=cu, status=status, **kw)
+    assert int(status) == 1 and float(got[5].abs().max()) == 0.0 and float(got[265].abs().max()) == 0.0
 
 
 @pytest.mark.parametrize("dtype", TYPES)
