@@ -17,6 +17,8 @@
 // Bound by the exponentials (16 a clock and SM: 1024 clocks per 128 x 128 tile) and, at head_dim 128, equally by the products.
 // Every wait is bounded; on expiry the block sets *status, frees its tensor memory and returns.
 #pragma once
+#include <type_traits>
+
 #include "attn_kv8.cuh"
 #include "tc_ptx.cuh"
 
@@ -24,14 +26,15 @@ namespace sllm {
 
 constexpr int kT8Rows = 128;                     // query rows of a tile
 constexpr int kT8Keys = 128;                     // keys of a step
-constexpr int kT8SoftWarps = 8, kT8WideWarps = 4;
-constexpr int kT8Threads = (kT8SoftWarps + kT8WideWarps + 1) * 32;
 constexpr int kT8Blks = kT8Keys / kBlk8;         // scale blocks of a step
 constexpr int kT8Ring = 4;                       // steps whose scales are held
 constexpr float kT8Slack = 8.f;                  // log2 units that scores may pass m by
+constexpr int kT8MaxSort = 256;                  // sequences up to which blocks order the tiles by their keys
 
-template <int HD> __host__ __device__ constexpr size_t attn8_tc_smem() {
-    return 1024 + 2 * (size_t)kT8Rows * HD * 2 + 4 * (size_t)kT8Keys * HD * 2 + kT8Ring * (kT8Blks + 1) * 16 + 256;
+// NT tiles of query rows per block, 4 NT softmax warps, WW widening warps, one MMA warp
+template <int NT, int WW> __host__ __device__ constexpr int attn8_tc_threads() { return (4 * NT + WW + 1) * 32; }
+template <int HD, int NT> __host__ __device__ constexpr size_t attn8_tc_smem() {
+    return 1024 + NT * (size_t)kT8Rows * HD * 2 + 4 * (size_t)kT8Keys * HD * 2 + kT8Ring * (kT8Blks + 1) * 16 + 256;
 }
 
 __device__ __forceinline__ bool wait8(uint32_t bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, kWaitLimitNs); }
@@ -45,42 +48,108 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r) {
                  ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
                    "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
+__device__ __forceinline__ void tc_ld32_async(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr));
+}
+// waits for the loads so far; the registers they fill pass through, so that no use of them moves in front of it
+__device__ __forceinline__ void tc_wait_ld64(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(r[i]));
+}
+// two floats at a time: a * b + c, a + b
+__device__ __forceinline__ unsigned long long pair2(float a, float b) {
+    unsigned long long x;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
+    return x;
+}
+__device__ __forceinline__ float2 unpair2(unsigned long long x) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(x));
+    return f;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-template <int HD>
-__global__ void __launch_bounds__(kT8Threads, 1) k_attn_kv8_tc(const Attn8Args a) {
+template <int HD, int NT, int WW>
+__global__ void __launch_bounds__(attn8_tc_threads<NT, WW>(), NT == 1 ? 2 : 1) k_attn_kv8_tc(const Attn8Args a) {
+    constexpr int SOFT = 4 * NT;                              // softmax warps 0 .. SOFT - 1, then the widening ones, then the MMA warp
+    constexpr int THREADS = attn8_tc_threads<NT, WW>();
+    constexpr uint32_t TMEM_COLS = NT * (kT8Keys + HD) > 256 ? 512 : 256;
     constexpr int HALVES = HD / 64;                           // 128-byte column blocks of a row
     constexpr uint32_t HALF = kT8Keys * 128;                  // bytes of one of them (query rows and keys are both 128)
     constexpr uint32_t TILE = HALVES * HALF;
     constexpr int CPR = HD / 16;                              // 16-byte chunks of int8 per cache row
-    constexpr int RPP = kT8WideWarps * 32 / CPR;              // rows per pass of the widening threads
+    constexpr int RPP = WW * 32 / CPR;              // rows per pass of the widening threads
     constexpr int PASSES = kT8Keys / RPP;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* sQ = smem;                                       // [2][TILE]
-    uint8_t* sK = sQ + 2 * TILE;                              // [2 stages][TILE]
+    uint8_t* sK = sQ + NT * TILE;                              // [2 stages][TILE]
     uint8_t* sV = sK + 2 * TILE;
     float4* s_blk = reinterpret_cast<float4*>(sV + 2 * TILE); // [ring][blocks]: c, log2 v, 1 / v, 0 or -inf (blocks that do not count)
     float4* s_vr = s_blk + kT8Ring * kT8Blks;                 // [ring]: vr
     uint64_t* bars = reinterpret_cast<uint64_t*>(s_vr + kT8Ring);
     enum { K_FULL = 0, V_FULL = 2, K_FREE = 4, V_FREE = 6, S_READY = 8, P_READY = 10, SC_FULL = 12, O_DONE = 16, N_BARS = 17 };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
-    __shared__ int s_last[kT8SoftWarps];
+    __shared__ int s_last[8];
+    __shared__ int s_len[kT8MaxSort], s_tiles[kT8MaxSort], s_pick[2];
     const uint32_t bar0 = smem_u32(bars);
     auto B = [&](int i) { return bar0 + 8u * (uint32_t)i; };
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_launch_dependents();
     pdl_wait();
-    int t0, seq;
-    const int n = attn8_tile(a, gridDim.x - 1 - blockIdx.x, t0, seq);      // late tiles, which have the most keys, first
+    // Which tile: those with the most keys first, so that the last blocks to start are short ones.  With few sequences each
+    // block sorts them by their last position (the tiles of one are near one another); with many, the grid is long anyway.
+    int t0 = 0, seq = 0, n = 0;
+    if (a.n_seq <= kT8MaxSort) {
+        if (tid == 0) s_pick[0] = -1;
+        for (int i = tid; i < a.n_seq; i += THREADS) {
+            const int c0 = a.cu_tok[i], c1 = min(a.cu_tok[i + 1], a.n_tok);
+            const bool any = c0 >= 0 && c1 > c0;
+            s_tiles[i] = any ? (c1 - c0 + a.rows_toks - 1) / a.rows_toks : 0;
+            s_len[i] = any ? a.tok_pos[c1 - 1] : -1;
+        }
+        __syncthreads();
+        for (int i = tid; i < a.n_seq; i += THREADS) {
+            int before = 0;
+            const int len = s_len[i];
+            for (int j = 0; j < a.n_seq; ++j) before += s_len[j] > len || (s_len[j] == len && j < i) ? s_tiles[j] : 0;
+            const int k = (int)blockIdx.y - before;
+            if (k >= 0 && k < s_tiles[i]) { s_pick[0] = i; s_pick[1] = s_tiles[i] - 1 - k; }
+        }
+        __syncthreads();
+        seq = s_pick[0];
+        if (seq >= 0) {
+            const int c0 = a.cu_tok[seq];
+            t0 = c0 + s_pick[1] * a.rows_toks;
+            n = min(a.rows_toks, min(a.cu_tok[seq + 1], a.n_tok) - t0);
+        }
+    } else n = attn8_tile(a, gridDim.y - 1 - blockIdx.y, t0, seq);
     if (n <= 0) return;
-    const int head = blockIdx.y, group = a.group, toks = a.rows_toks >> 1; // tokens of one tile
+    const int head = blockIdx.x, group = a.group, toks = a.rows_toks / NT;   // tokens of one tile
     const int most = (int)min((long long)a.width * kPage, 0x7fffff00ll) - 1;
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(B(K_FULL + i), kT8WideWarps); mbar_init(B(V_FULL + i), kT8WideWarps);
+            mbar_init(B(K_FULL + i), WW); mbar_init(B(V_FULL + i), WW);
             mbar_init(B(K_FREE + i), 1); mbar_init(B(V_FREE + i), 1);
             mbar_init(B(S_READY + i), 1); mbar_init(B(P_READY + i), 4);
         }
@@ -88,8 +157,8 @@ __global__ void __launch_bounds__(kT8Threads, 1) k_attn_kv8_tc(const Attn8Args a
         mbar_init(B(O_DONE), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kT8SoftWarps + kT8WideWarps) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+    if (warp == SOFT + WW) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
 
@@ -97,7 +166,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) k_attn_kv8_tc(const Attn8Args a
     const int tile = warp >> 2, r = tid & 127;                // of the softmax warps
     int pos = 0, row_tok = -1, row_head = 0;
     float row_f = 0.f;
-    if (warp < kT8SoftWarps) {
+    if (warp < SOFT) {
         const int rt = tile * toks + r / group;
         const bool valid = r / group < toks && rt < n;
         if (valid) { row_tok = t0 + rt; row_head = head * group + r % group; }
@@ -143,12 +212,12 @@ __global__ void __launch_bounds__(kT8Threads, 1) k_attn_kv8_tc(const Attn8Args a
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int last0 = max(max(s_last[0], s_last[1]), max(s_last[2], s_last[3]));
-    const int last1 = max(max(s_last[4], s_last[5]), max(s_last[6], s_last[7]));
+    const int last1 = NT == 2 ? max(max(s_last[4], s_last[5]), max(s_last[6], s_last[7])) : -1;
     const int last = max(last0, last1);
     const int n0 = (last0 + kT8Keys) / kT8Keys, n1 = (last1 + kT8Keys) / kT8Keys, steps = max(n0, n1);     // 0 where nothing is attended
     bool ok = true;
 
-    if (warp == kT8SoftWarps + kT8WideWarps) {
+    if (warp == SOFT + WW) {
         // ---- MMA ----
         if (lane == 0) {
             const uint32_t id_s = (1u << 4) | ((uint32_t)(kT8Keys >> 3) << 17) | ((uint32_t)(kT8Rows >> 4) << 24);     // fp16 x fp16 -> fp32
@@ -168,7 +237,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) k_attn_kv8_tc(const Attn8Args a
                 for (int h = 0; h < HALVES; ++h)
 #pragma unroll
                     for (int j = 0; j < kT8Keys / 16; ++j)
-                        tc_mma_f16_ts(tmem + 2 * kT8Keys + t * HD + h * 64, tmem + (uint32_t)(t * kT8Keys + j * 8), tc_smem_desc(v + h * HALF + j * 2048), id_o, i > 0 || j > 0);
+                        tc_mma_f16_ts(tmem + NT * kT8Keys + t * HD + h * 64, tmem + (uint32_t)(t * kT8Keys + j * 8), tc_smem_desc(v + h * HALF + j * 2048), id_o, i > 0 || j > 0);
             };
             if (steps > 0) {
                 ok = wait8(B(K_FULL), 0);
@@ -180,7 +249,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) k_attn_kv8_tc(const Attn8Args a
             for (int i = 0; i < steps && ok; ++i) {
                 const int s = i & 1;
                 ok = wait8(B(V_FULL + s), (i >> 1) & 1);
-                for (int t = 0; t < 2 && ok; ++t) {
+                for (int t = 0; t < NT && ok; ++t) {
                     const int nt = t ? n1 : n0;
                     if (i < nt) {
                         ok = wait8(B(P_READY + t), i & 1);
@@ -201,9 +270,9 @@ __global__ void __launch_bounds__(kT8Threads, 1) k_attn_kv8_tc(const Attn8Args a
             }
             if (ok && steps > 0) tc_commit(B(O_DONE));
         }
-    } else if (warp >= kT8SoftWarps) {
+    } else if (warp >= SOFT) {
         // ---- widening: int8 rows -> fp16 tiles, and the blocks' factors ----
-        const int w = tid - kT8SoftWarps * 32, c = w % CPR, row0 = w / CPR;
+        const int w = tid - SOFT * 32, c = w % CPR, row0 = w / CPR;
         const int* table = a.table + (size_t)seq * a.width;
         const int8_t* pool = a.c.pages;
         auto page_of = [&](int i, int half) -> int {          // -1: behind the last position, -2: outside the pool
@@ -290,82 +359,106 @@ __global__ void __launch_bounds__(kT8Threads, 1) k_attn_kv8_tc(const Attn8Args a
     } else {
         // ---- softmax: thread = query row = TMEM lane ----
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t s_at = lanes + tile * kT8Keys, o_at = lanes + 2 * kT8Keys + tile * HD;
+        const uint32_t s_at = lanes + tile * kT8Keys, o_at = lanes + NT * kT8Keys + tile * HD;
         const int my_steps = tile ? n1 : n0;
         const int open = row_tok >= 0 ? pos : 0x7fffffff;      // rows of no token: q = 0, whatever they come to is not written
         const int all_see = __reduce_min_sync(0xffffffffu, open);
         float m = -INFINITY, l = 0.f, vr = 0.f;
+        // One step, 64 keys at a time so that their scores stay in registers: maximum, weights, and the weights over the scores.
+        auto half_steps = [&](auto masked, const float4* blk, float vr_now, int kb, bool have_o) {
+            constexpr bool MASKED = decltype(masked)::value;
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+                uint32_t sv[64];
+                tc_ld32_async(s_at + h * 64, sv);
+                tc_ld32_async(s_at + h * 64 + 32, sv + 32);
+                tc_wait_ld64(sv);
+                const int k0 = kb + h * 64;
+                if (MASKED) {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j)
+                        if (k0 + j > open) sv[j] = 0xff800000u;
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    float t4[2] = {__uint_as_float(sv[b * 16]), __uint_as_float(sv[b * 16 + 1])};
+#pragma unroll
+                    for (int j = 2; j < 16; j += 4) {
+                        t4[0] = fmaxf(fmaxf(t4[0], __uint_as_float(sv[b * 16 + j])), __uint_as_float(sv[b * 16 + j + 1]));
+                        if (j + 2 < 16) t4[1] = fmaxf(fmaxf(t4[1], __uint_as_float(sv[b * 16 + j + 2])), __uint_as_float(sv[b * 16 + j + 3]));
+                    }
+                    const float4 f = blk[h * 4 + b];
+                    mx = fmaxf(mx, fmaf(fmaxf(t4[0], t4[1]), f.x * row_f, f.w));
+                }
+                const bool moves = mx > m + kT8Slack || (m == -INFINITY && mx > m);
+                if (__any_sync(0xffffffffu, moves || vr_now != vr)) {
+                    const float m_new = moves ? mx : m;
+                    const float corr = m == -INFINITY ? 0.f : exp2_fast(m - m_new);
+                    l *= corr;
+                    uint32_t x[16];
+                    if (have_o) {                              // every product into O so far is done: S of this step came after them
+                        const float f = corr * (vr_now > 0.f ? vr / vr_now : 1.f);
+#pragma unroll 1
+                        for (int c = 0; c < HD / 16; ++c) {
+                            tc_ld16(o_at + c * 16, x);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * f);
+                            tc_st16(o_at + c * 16, x);
+                        }
+                    }
+                    if (h == 1) {                              // the weights of this step's first half are relative to the old m
+                        tc_wait_st();
+#pragma unroll 1
+                        for (int c = 0; c < 2; ++c) {
+                            tc_ld16(s_at + c * 16, x);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&x[j]));
+                                x[j] = pack_half(w.x * corr, w.y * corr);
+                            }
+                            tc_st16(s_at + c * 16, x);
+                        }
+                    }
+                    m = m_new;
+                    vr = vr_now;
+                }
+                const float m_use = m == -INFINITY ? 0.f : m;
+                uint32_t pk[32];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const float4 f = blk[h * 4 + b];
+                    const float c = f.x * row_f, d = f.y - m_use;
+                    const unsigned long long c2 = pair2(c, c), d2 = pair2(d, d);
+                    unsigned long long sum = 0;
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        const float2 x = unpair2(fma2(pair2(__uint_as_float(sv[b * 16 + j]), __uint_as_float(sv[b * 16 + j + 1])), c2, d2));
+                        float w0 = exp2_fast(x.x), w1 = exp2_fast(x.y);
+                        if (MASKED) {                          // also where a factor is NaN
+                            if (k0 + b * 16 + j > open) w0 = 0.f;
+                            if (k0 + b * 16 + j + 1 > open) w1 = 0.f;
+                        }
+                        sum = add2(sum, pair2(w0, w1));
+                        pk[b * 8 + j / 2] = pack_half(w0, w1);
+                    }
+                    const float2 s2 = unpair2(sum);
+                    l = fmaf(s2.x + s2.y, f.z, l);
+                }
+                tc_st16(s_at + h * 32, pk);                    // over columns of S that this thread has read
+                tc_st16(s_at + h * 32 + 16, pk + 16);
+            }
+        };
         for (int i = 0; i < my_steps && ok; ++i) {
             ok = wait8(B(SC_FULL + i % kT8Ring), (i / kT8Ring) & 1) && wait8(B(S_READY + tile), i & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
             const float4* blk = s_blk + (i % kT8Ring) * kT8Blks;
-            const int kb = i * kT8Keys;
-            const bool masked = kb + kT8Keys - 1 > all_see;    // the same for the whole warp
-            uint32_t sv[32];
-            float mx = -INFINITY;
-#pragma unroll
-            for (int h = 0; h < kT8Keys / 32; ++h) {
-                tc_ld32(s_at + h * 32, sv);
-                if (masked) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (kb + h * 32 + j > open) sv[j] = 0xff800000u;
-                }
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    float t4[4] = {__uint_as_float(sv[b * 16]), __uint_as_float(sv[b * 16 + 1]), __uint_as_float(sv[b * 16 + 2]), __uint_as_float(sv[b * 16 + 3])};
-#pragma unroll
-                    for (int j = 4; j < 16; ++j) t4[j & 3] = fmaxf(t4[j & 3], __uint_as_float(sv[b * 16 + j]));
-                    const float4 f = blk[h * 2 + b];
-                    mx = fmaxf(mx, fmaf(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])), f.x * row_f, f.w));
-                }
-            }
             const float vr_now = s_vr[i % kT8Ring].x;
-            const bool moves = mx > m + kT8Slack || (m == -INFINITY && mx > m);
-            if (__any_sync(0xffffffffu, moves || vr_now != vr)) {
-                const float m_new = moves ? mx : m;
-                const float corr = m == -INFINITY ? 0.f : exp2_fast(m - m_new);
-                l *= corr;
-                if (i > 0) {                                   // every product into O so far is done: S of this step came after them
-                    const float f = corr * (vr_now > 0.f ? vr / vr_now : 1.f);
-#pragma unroll
-                    for (int h = 0; h < HD / 16; ++h) {
-                        tc_ld16(o_at + h * 16, sv);
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) sv[j] = __float_as_uint(__uint_as_float(sv[j]) * f);
-                        tc_st16(o_at + h * 16, sv);
-                    }
-                }
-                m = m_new;
-                vr = vr_now;
-            }
-            const float m_use = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int h = 0; h < kT8Keys / 32; ++h) {
-                tc_ld32(s_at + h * 32, sv);
-                uint32_t pk[16];
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const float4 f = blk[h * 2 + b];
-                    const float c = f.x * row_f, d = f.y - m_use;
-                    float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        float w0 = exp2_fast(fmaf(__uint_as_float(sv[b * 16 + j]), c, d));
-                        float w1 = exp2_fast(fmaf(__uint_as_float(sv[b * 16 + j + 1]), c, d));
-                        if (masked) {
-                            if (kb + h * 32 + b * 16 + j > open) w0 = 0.f;
-                            if (kb + h * 32 + b * 16 + j + 1 > open) w1 = 0.f;
-                        }
-                        sum0 += w0; sum1 += w1;
-                        pk[b * 8 + j / 2] = pack_half(w0, w1);
-                    }
-                    l = fmaf(sum0 + sum1, f.z, l);
-                }
-                tc_st16(s_at + h * 16, pk);                    // over columns of S that this thread has read
-            }
+            const int kb = i * kT8Keys;
+            if (kb + kT8Keys - 1 > all_see) half_steps(std::integral_constant<bool, true>{}, blk, vr_now, kb, i > 0);
+            else half_steps(std::integral_constant<bool, false>{}, blk, vr_now, kb, i > 0);
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -391,9 +484,9 @@ __global__ void __launch_bounds__(kT8Threads, 1) k_attn_kv8_tc(const Attn8Args a
     if (!ok && a.status) atomicExch(a.status, 5);
     tc_fence_before();
     __syncthreads();
-    if (warp == kT8SoftWarps + kT8WideWarps) {
+    if (warp == SOFT + WW) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
     }
 }
 
