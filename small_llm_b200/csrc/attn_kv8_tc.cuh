@@ -31,17 +31,35 @@ constexpr int kT8Ring = 4;                       // steps whose scales are held
 constexpr float kT8Slack = 8.f;                  // log2 units that scores may pass m by
 constexpr int kT8MaxSort = 256;                  // sequences up to which blocks order the tiles by their keys
 
-// NT tiles of query rows per block, 4 NT softmax warps, WW widening warps, one MMA warp
-template <int NT, int WW> __host__ __device__ constexpr int attn8_tc_threads() { return (4 * NT + WW + 1) * 32; }
+// NT tiles of query rows per block.  Warps: 4 NT softmax; 4 widening K and 4 widening V (NT = 1: 4 for both); the last four are
+// the MMA warp, the scales' warp and two that idle.  Registers are dealt out again at the start (setmaxnreg): the launch has
+// 640 x 96 = 61440 (NT = 1: 384 x 80 = 30720 per block, two blocks), of which the softmax takes 256 x 144 (128 x 136), the
+// widening 256 x 72 (128 x 64) and the last four warps 128 x 48 (128 x 40): 61440 (30720).
+template <int NT> __host__ __device__ constexpr int attn8_tc_threads() { return NT == 2 ? 640 : 384; }
 template <int HD, int NT> __host__ __device__ constexpr size_t attn8_tc_smem() {
     return 1024 + NT * (size_t)kT8Rows * HD * 2 + 4 * (size_t)kT8Keys * HD * 2 + kT8Ring * (kT8Blks + 1) * 16 + 256;
 }
 
 __device__ __forceinline__ bool wait8(uint32_t bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, kWaitLimitNs); }
-__device__ __forceinline__ void tc_mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-                 ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(acc) : "memory");
+// One lane of a converged warp.  The loop around it stays the same for all lanes, so that addresses and descriptors are kept in
+// uniform registers, where the instruction wants them (a loop run by one lane alone spent about 100 cycles on each).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
+}
+// Operand descriptors differ in their low words only, so those are what is kept and added to.
+constexpr uint32_t kT8DescHi = (uint32_t)(64u | 1u << 14 | 2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(const void* p) { return ((smem_u32(p) >> 4) & 0x3fff) | 1u << 16; }
+__device__ __forceinline__ void tc_mma_f16_ss(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 x, y;\nsetp.ne.b32 p, %4, 0;\nmov.b64 x, {%1, %5};\nmov.b64 y, {%2, %5};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}"
+                 ::"r"(tmem_d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kT8DescHi) : "memory");
+}
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 y;\nsetp.ne.b32 p, %4, 0;\nmov.b64 y, {%2, %5};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}"
+                 ::"r"(tmem_d), "r"(tmem_a), "r"(b), "r"(idesc), "r"(acc), "n"(kT8DescHi) : "memory");
 }
 __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -87,16 +105,19 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-template <int HD, int NT, int WW>
-__global__ void __launch_bounds__(attn8_tc_threads<NT, WW>(), NT == 1 ? 2 : 1) k_attn_kv8_tc(const Attn8Args a) {
-    constexpr int SOFT = 4 * NT;                              // softmax warps 0 .. SOFT - 1, then the widening ones, then the MMA warp
-    constexpr int THREADS = attn8_tc_threads<NT, WW>();
+template <int R> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_attn_kv8_tc(const Attn8Args a) {
+    constexpr int SOFT = 4 * NT, WIDE = 4 * NT;               // softmax warps 0 .. SOFT - 1, then the widening ones, MMA, scales
+    constexpr int THREADS = attn8_tc_threads<NT>();
     constexpr uint32_t TMEM_COLS = NT * (kT8Keys + HD) > 256 ? 512 : 256;
     constexpr int HALVES = HD / 64;                           // 128-byte column blocks of a row
     constexpr uint32_t HALF = kT8Keys * 128;                  // bytes of one of them (query rows and keys are both 128)
     constexpr uint32_t TILE = HALVES * HALF;
     constexpr int CPR = HD / 16;                              // 16-byte chunks of int8 per cache row
-    constexpr int RPP = WW * 32 / CPR;              // rows per pass of the widening threads
+    constexpr int RPP = 128 / CPR;              // rows per pass of the widening threads
     constexpr int PASSES = kT8Keys / RPP;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -106,9 +127,9 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT, WW>(), NT == 1 ? 2 : 1) k
     float4* s_blk = reinterpret_cast<float4*>(sV + 2 * TILE); // [ring][blocks]: c, log2 v, 1 / v, 0 or -inf (blocks that do not count)
     float4* s_vr = s_blk + kT8Ring * kT8Blks;                 // [ring]: vr
     uint64_t* bars = reinterpret_cast<uint64_t*>(s_vr + kT8Ring);
-    enum { K_FULL = 0, V_FULL = 2, K_FREE = 4, V_FREE = 6, S_READY = 8, P_READY = 10, SC_FULL = 12, O_DONE = 16, N_BARS = 17 };
+    enum { K_FULL = 0, V_FULL = 2, K_FREE = 4, V_FREE = 6, S_READY = 8, P_READY = 10, SC_FULL = 12, O_DONE = 16, Q_FULL = 17, N_BARS = 18 };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
-    __shared__ int s_last[8];
+    __shared__ int s_last[2][8];
     __shared__ int s_len[kT8MaxSort], s_tiles[kT8MaxSort], s_pick[2];
     const uint32_t bar0 = smem_u32(bars);
     auto B = [&](int i) { return bar0 + 8u * (uint32_t)i; };
@@ -149,215 +170,252 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT, WW>(), NT == 1 ? 2 : 1) k
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(B(K_FULL + i), WW); mbar_init(B(V_FULL + i), WW);
+            mbar_init(B(K_FULL + i), 4); mbar_init(B(V_FULL + i), 4);
             mbar_init(B(K_FREE + i), 1); mbar_init(B(V_FREE + i), 1);
             mbar_init(B(S_READY + i), 1); mbar_init(B(P_READY + i), 4);
         }
         for (int i = 0; i < kT8Ring; ++i) mbar_init(B(SC_FULL + i), 1);
-        mbar_init(B(O_DONE), 1);
+        mbar_init(B(O_DONE), 1); mbar_init(B(Q_FULL), SOFT);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == SOFT + WW) {
+    if (warp == SOFT + WIDE) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
 
-    // the softmax threads' rows, and Q as fp16, K-major with the 128-byte swizzle; rows of no token are zero
-    const int tile = warp >> 2, r = tid & 127;                // of the softmax warps
-    int pos = 0, row_tok = -1, row_head = 0;
-    float row_f = 0.f;
-    if (warp < SOFT) {
-        const int rt = tile * toks + r / group;
-        const bool valid = r / group < toks && rt < n;
-        if (valid) { row_tok = t0 + rt; row_head = head * group + r % group; }
-        pos = valid ? min(a.tok_pos[row_tok], most) : -1;
-        const int last_w = __reduce_max_sync(0xffffffffu, pos);
-        if (lane == 0) s_last[warp] = last_w;
-        uint4 raw[HD / 8];
-        const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + (valid ? (long long)row_tok * a.q_stride + row_head * HD : 0);
-        unsigned top = 0;
-#pragma unroll
-        for (int c = 0; c < HD / 8; ++c) {
-            raw[c] = make_uint4(0u, 0u, 0u, 0u);
-            if (valid) {
-                if (a.wide) raw[c] = *reinterpret_cast<const uint4*>(src + 8 * c);
-                else {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        w[j] = (uint32_t)__bfloat16_as_ushort(src[8 * c + 2 * j]) | (uint32_t)__bfloat16_as_ushort(src[8 * c + 2 * j + 1]) << 16;
-                    raw[c] = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            }
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[c]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) top = max(top, max((w[j] & 0x7fffu) << 16, w[j] & 0x7fff0000u));
-        }
-        // f = 2^-e with the largest value in [2^(e-1), 2^e), as in the general kernel
-        const int e = min(max((int)(top >> 23) - 126, -125), 125);
-        const float f = top ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
-        row_f = top ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
-        const float fs = a.scale < 0.f ? -f : f;              // block factors are positive: a maximum may be taken before them
-#pragma unroll
-        for (int c = 0; c < HD / 8; ++c) {
-            float x[8];
-            unpack16<__nv_bfloat16>(raw[c], x);
-            *reinterpret_cast<uint4*>(sQ + tile * TILE + (c >> 3) * HALF + sw128(r, c & 7)) =
-                make_uint4(pack_half(x[0] * fs, x[1] * fs), pack_half(x[2] * fs, x[3] * fs), pack_half(x[4] * fs, x[5] * fs), pack_half(x[6] * fs, x[7] * fs));
-        }
-        fence_async_smem();
+    // last position of each tile's tokens
+    if (tid < 2 * kT8Rows) {
+        const int pos = tid < n ? min(a.tok_pos[t0 + tid], most) : -1;
+        const int p0 = __reduce_max_sync(0xffffffffu, tid < toks ? pos : -1), p1 = __reduce_max_sync(0xffffffffu, tid < toks ? -1 : pos);
+        if (lane == 0) { s_last[0][warp] = p0; s_last[1][warp] = p1; }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
-    const int last0 = max(max(s_last[0], s_last[1]), max(s_last[2], s_last[3]));
-    const int last1 = NT == 2 ? max(max(s_last[4], s_last[5]), max(s_last[6], s_last[7])) : -1;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    int last0 = -1, last1 = -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { last0 = max(last0, s_last[0][i]); last1 = max(last1, s_last[1][i]); }
     const int last = max(last0, last1);
     const int n0 = (last0 + kT8Keys) / kT8Keys, n1 = (last1 + kT8Keys) / kT8Keys, steps = max(n0, n1);     // 0 where nothing is attended
     bool ok = true;
 
-    if (warp == SOFT + WW) {
+    const int* table = a.table + (size_t)seq * a.width;
+    auto page_of = [&](int i, int half) -> int {              // page of a step's first or second 64 keys; -1: behind the last position, -2: outside the pool
+        const int p = 2 * i + half;
+        if ((long long)p * kPage > last) return -1;
+        const int id = table[p];
+        return id < 0 || id >= a.c.n_pages ? -2 : id;
+    };
+    if (warp >= SOFT + WIDE) {
+        fewer_registers<NT == 2 ? 48 : 40>();
+        if (warp == SOFT + WIDE) {
         // ---- MMA ----
-        if (lane == 0) {
-            const uint32_t id_s = (1u << 4) | ((uint32_t)(kT8Keys >> 3) << 17) | ((uint32_t)(kT8Rows >> 4) << 24);     // fp16 x fp16 -> fp32
-            const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(kT8Rows >> 4) << 24);   // V: MN-major
-            auto issue_s = [&](int i, int t) {
-                const uint32_t q = smem_u32(sQ) + t * TILE, k = smem_u32(sK) + (i & 1) * TILE;
+        const uint32_t id_s = (1u << 4) | ((uint32_t)(kT8Keys >> 3) << 17) | ((uint32_t)(kT8Rows >> 4) << 24);     // fp16 x fp16 -> fp32
+        const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(kT8Rows >> 4) << 24);   // V: MN-major
+        // descriptors of the first tiles; a place further on is its distance / 16 more
+        const uint32_t q_desc = desc_lo(sQ), k_desc = desc_lo(sK), v_desc = desc_lo(sV);
+        auto issue_s = [&](int i, int t) {
+            const uint32_t q = q_desc + (uint32_t)t * (TILE / 16), k = k_desc + (uint32_t)(i & 1) * (TILE / 16);
+            if (elect_one()) {
 #pragma unroll
                 for (int j = 0; j < HD / 16; ++j) {
-                    const uint32_t at = (j >> 2) * HALF + (j & 3) * 32;
-                    tc_mma_bf16(tmem + (uint32_t)(t * kT8Keys), tc_smem_desc(q + at), tc_smem_desc(k + at), id_s, j != 0);
+                    const uint32_t at = ((j >> 2) * HALF + (j & 3) * 32) / 16;
+                    tc_mma_f16_ss(tmem + (uint32_t)(t * kT8Keys), q + at, k + at, id_s, j != 0);
                 }
                 tc_commit(B(S_READY + t));
-            };
-            auto issue_o = [&](int i, int t) {
-                const uint32_t v = smem_u32(sV) + (i & 1) * TILE;
+            }
+            __syncwarp();
+        };
+        auto issue_o = [&](int i, int t) {
+            const uint32_t v = v_desc + (uint32_t)(i & 1) * (TILE / 16);
+            if (elect_one()) {
 #pragma unroll
                 for (int h = 0; h < HALVES; ++h)
 #pragma unroll
                     for (int j = 0; j < kT8Keys / 16; ++j)
-                        tc_mma_f16_ts(tmem + NT * kT8Keys + t * HD + h * 64, tmem + (uint32_t)(t * kT8Keys + j * 8), tc_smem_desc(v + h * HALF + j * 2048), id_o, i > 0 || j > 0);
-            };
-            if (steps > 0) {
-                ok = wait8(B(K_FULL), 0);
-                tc_fence_after();
-                if (ok && n0 > 0) issue_s(0, 0);
-                if (ok && n1 > 0) issue_s(0, 1);
-                if (ok) tc_commit(B(K_FREE));
+                        tc_mma_f16_ts(tmem + NT * kT8Keys + t * HD + h * 64, tmem + (uint32_t)(t * kT8Keys + j * 8), v + (h * HALF + j * 2048) / 16, id_o, i > 0 || j > 0);
             }
-            for (int i = 0; i < steps && ok; ++i) {
-                const int s = i & 1;
-                ok = wait8(B(V_FULL + s), (i >> 1) & 1);
-                for (int t = 0; t < NT && ok; ++t) {
-                    const int nt = t ? n1 : n0;
-                    if (i < nt) {
-                        ok = wait8(B(P_READY + t), i & 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        issue_o(i, t);
-                    }
-                    if (i + 1 < nt) {
-                        ok = wait8(B(K_FULL + (s ^ 1)), ((i + 1) >> 1) & 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        issue_s(i + 1, t);
-                    }
+            __syncwarp();
+        };
+        auto commit = [&](int bar) { if (elect_one()) tc_commit(B(bar)); __syncwarp(); };
+        // A wait that gives up does so in every lane or soon after: the warp goes on as one.
+        auto wait = [&](int bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, wait8(B(bar), parity)); };
+        if (steps > 0) {
+            ok = wait(Q_FULL, 0) && wait(K_FULL, 0);
+            tc_fence_after();
+            if (ok && n0 > 0) issue_s(0, 0);
+            if (ok && n1 > 0) issue_s(0, 1);
+            if (ok) commit(K_FREE);
+        }
+        for (int i = 0; i < steps && ok; ++i) {
+            const int s = i & 1;
+            ok = wait(V_FULL + s, (i >> 1) & 1);
+            for (int t = 0; t < NT && ok; ++t) {
+                const int nt = t ? n1 : n0;
+                if (i < nt) {
+                    ok = wait(P_READY + t, i & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_o(i, t);
                 }
-                if (!ok) break;
-                tc_commit(B(V_FREE + s));
-                if (i + 1 < steps) tc_commit(B(K_FREE + (s ^ 1)));
+                if (i + 1 < nt) {
+                    ok = wait(K_FULL + (s ^ 1), ((i + 1) >> 1) & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_s(i + 1, t);
+                }
             }
-            if (ok && steps > 0) tc_commit(B(O_DONE));
+            if (!ok) break;
+            commit(V_FREE + s);
+            if (i + 1 < steps) commit(K_FREE + (s ^ 1));
+        }
+        if (ok && steps > 0) commit(O_DONE);
+        } else if (warp == SOFT + WIDE + 1) {
+        // ---- the blocks' factors: lane b takes block b of a step; the loads are a step ahead ----
+        float ks = 0.f, vs = 0.f, vr = 0.f;
+        bool counts = false;
+        int id = lane < kT8Blks && steps > 0 ? page_of(0, lane / kBlksPerPage) : -1;
+        auto fetch = [&](int i) {
+            counts = id >= 0 && (long long)i * kT8Keys + lane * kBlk8 <= last;
+            if (id == -2 && a.status) atomicExch(a.status, 1);
+            if (counts) {
+                const float* sc = a.c.scales + ((long long)id * a.c.H + head) * 2 * kBlksPerPage + (lane % kBlksPerPage);
+                ks = sc[0]; vs = sc[kBlksPerPage];
+            }
+        };
+        if (steps > 0) fetch(0);
+        for (int i = 0; i < steps && ok; ++i) {
+            id = lane < kT8Blks && i + 1 < steps ? page_of(i + 1, lane / kBlksPerPage) : -1;
+            float top = counts && vs == vs ? vs : 0.f;
+#pragma unroll
+            for (int o = 1; o < kT8Blks; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (top > vr) vr = pow2_above(fminf(top, 1.7e38f));
+            const float v0 = vr > 0.f ? vs / vr : (vs == 0.f ? 1.f : vs);
+            const float v = v0 != v0 ? v0 : fmaxf(v0, 8.67361738e-19f);              // 2^-60: fp16 takes such a weight for 0, the sum does not
+            const float4 f = counts ? make_float4(ks * fabsf(a.scale) * 1.4426950408889634f, log2f(v), 1.f / v, 0.f) : make_float4(0.f, -INFINITY, 0.f, -INFINITY);
+            // step i - 2's K is free: the softmax is done with step i - 3, whose place in the ring may be written
+            if (i >= 2) ok = __all_sync(0xffffffffu, wait8(B(K_FREE + (i & 1)), ((i >> 1) - 1) & 1));
+            if (!ok) break;
+            if (lane < kT8Blks) s_blk[(i % kT8Ring) * kT8Blks + lane] = f;
+            if (lane == 0) s_vr[i % kT8Ring].x = vr;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(B(SC_FULL + i % kT8Ring));
+            if (i + 1 < steps) fetch(i + 1);
+        }
         }
     } else if (warp >= SOFT) {
-        // ---- widening: int8 rows -> fp16 tiles, and the blocks' factors ----
-        const int w = tid - SOFT * 32, c = w % CPR, row0 = w / CPR;
-        const int* table = a.table + (size_t)seq * a.width;
-        const int8_t* pool = a.c.pages;
-        auto page_of = [&](int i, int half) -> int {          // -1: behind the last position, -2: outside the pool
-            const int p = 2 * i + half;
-            if ((long long)p * kPage > last) return -1;
-            const int id = table[p];
-            if (id < 0 || id >= a.c.n_pages) { if (a.status && w == 0) atomicExch(a.status, 1); return -2; }
-            return id;
-        };
+        // ---- widening: int8 rows -> fp16 tiles, the loads a step ahead ----
+        if constexpr (NT == 2) fewer_registers<72>(); else fewer_registers<64>();
+        const int w = tid & 127, c = w % CPR, row0 = w / CPR;
+        static_assert(RPP % 8 == 0, "rows of a thread share their place in the swizzle");
+        // the two column blocks of head_dim 128 store the halves of a chunk in opposite order: no bank conflicts
+        const int swap = HALVES == 2 ? (c >> 2) & 1 : 0, ch = (2 * c) & 7;
+        const uint32_t at0 = (c >> 2) * HALF + sw128(row0, ch + swap), at1 = (c >> 2) * HALF + sw128(row0, ch + 1 - swap);
         auto fetch = [&](int p0, int p1, int which, uint4 (&x)[PASSES]) {
 #pragma unroll
-            for (int j = 0; j < PASSES; ++j) {
-                const int row = row0 + j * RPP, id = j < PASSES / 2 ? p0 : p1;
-                x[j] = make_uint4(0u, 0u, 0u, 0u);
-                if (id >= 0)
-                    x[j] = *reinterpret_cast<const uint4*>(pool + ((((long long)id * a.c.H + head) * 2 + which) * kPage + (row & (kPage - 1))) * HD + c * 16);
+            for (int h = 0; h < 2; ++h) {
+                const int id = h ? p1 : p0;
+                const int8_t* src = a.c.pages + (((long long)id * a.c.H + head) * 2 + which) * (kPage * HD) + row0 * HD + c * 16;
+#pragma unroll
+                for (int j = 0; j < PASSES / 2; ++j)
+                    x[h * (PASSES / 2) + j] = id >= 0 ? *reinterpret_cast<const uint4*>(src + j * RPP * HD) : make_uint4(0u, 0u, 0u, 0u);
             }
         };
-        auto widen = [&](uint8_t* dst, const uint4 (&x)[PASSES]) {
-            const int swap = HALVES == 2 ? (c >> 2) & 1 : 0;   // the two column blocks store their halves of a chunk in opposite order: no bank conflicts
+        auto widen = [&](uint8_t* dst, const uint4 (&x)[PASSES], int full) {
 #pragma unroll
             for (int j = 0; j < PASSES; ++j) {
-                const int row = row0 + j * RPP;
                 const uint32_t u[4] = {x[j].x ^ 0x80808080u, x[j].y ^ 0x80808080u, x[j].z ^ 0x80808080u, x[j].w ^ 0x80808080u};
                 const uint4 lo = make_uint4(halves(u[0], 0x4140), halves(u[0], 0x4342), halves(u[1], 0x4140), halves(u[1], 0x4342));
                 const uint4 hi = make_uint4(halves(u[2], 0x4140), halves(u[2], 0x4342), halves(u[3], 0x4140), halves(u[3], 0x4342));
-                uint8_t* base = dst + (c >> 2) * HALF;
-                const int ch = (2 * c) & 7;
-                *reinterpret_cast<uint4*>(base + sw128(row, ch + swap)) = swap ? hi : lo;
-                *reinterpret_cast<uint4*>(base + sw128(row, ch + 1 - swap)) = swap ? lo : hi;
+                *reinterpret_cast<uint4*>(dst + at0 + j * RPP * 128) = swap ? hi : lo;
+                *reinterpret_cast<uint4*>(dst + at1 + j * RPP * 128) = swap ? lo : hi;
             }
             fence_async_smem();
             __syncwarp();
+            if (lane == 0) mbar_arrive(B(full));
         };
-        uint4 xk[PASSES], xv[PASSES];
-        int p0 = -1, p1 = -1;
-        float vr = 0.f;
-        if (steps > 0) { p0 = page_of(0, 0); p1 = page_of(0, 1); fetch(p0, p1, 0, xk); }
-        for (int i = 0; i < steps && ok; ++i) {
-            const int s = i & 1;
-            // scales of this step's blocks: lane b of the first warp takes block b
-            float ks = 0.f, vs = 0.f;
-            bool counts = false;
-            if (w < kT8Blks) {
-                const int id = w < kBlksPerPage ? p0 : p1;
-                counts = id >= 0 && (long long)i * kT8Keys + w * kBlk8 <= last;
-                if (counts) {
-                    const float* sc = a.c.scales + ((long long)id * a.c.H + head) * 2 * kBlksPerPage + (w % kBlksPerPage);
-                    ks = sc[0]; vs = sc[kBlksPerPage];
-                }
+        auto freed = [&](int bar, int i) { return i < 2 || __all_sync(0xffffffffu, wait8(B(bar + (i & 1)), ((i >> 1) - 1) & 1)); };
+        if constexpr (NT == 2) {
+            const int which = (warp - SOFT) >> 2;
+            uint8_t* dst = which ? sV : sK;
+            const int full = which ? V_FULL : K_FULL, free = which ? V_FREE : K_FREE;
+            uint4 x[PASSES];
+            int p0 = -1, p1 = -1;
+            if (steps > 0) { p0 = page_of(0, 0); p1 = page_of(0, 1); fetch(p0, p1, which, x); }
+            for (int i = 0; i < steps && ok; ++i) {
+                const bool more = i + 1 < steps;
+                if (more) { p0 = page_of(i + 1, 0); p1 = page_of(i + 1, 1); }
+                ok = freed(free, i);
+                if (!ok) break;
+                widen(dst + (i & 1) * TILE, x, full + (i & 1));
+                if (more) fetch(p0, p1, which, x);
             }
-            fetch(p0, p1, 1, xv);
-            int q0 = -1, q1 = -1;
-            if (i + 1 < steps) { q0 = page_of(i + 1, 0); q1 = page_of(i + 1, 1); }
-            if (i >= 2) ok = wait8(B(K_FREE + s), ((i >> 1) - 1) & 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            if (w < 32) {
-                // K_FREE of step i - 2 means that the softmax is done with step i - 3: its place in the ring may be written
-                float top = counts && vs == vs ? vs : 0.f;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                if (top > vr) vr = pow2_above(fminf(top, 1.7e38f));
-                if (w < kT8Blks) {
-                    const float v0 = vr > 0.f ? vs / vr : (vs == 0.f ? 1.f : vs);
-                    const float v = v0 != v0 ? v0 : fmaxf(v0, 8.67361738e-19f);          // 2^-60: fp16 takes such a weight for 0, the sum does not
-                    s_blk[(i % kT8Ring) * kT8Blks + w] = counts ? make_float4(ks * fabsf(a.scale) * 1.4426950408889634f, log2f(v), 1.f / v, 0.f)
-                                                                : make_float4(0.f, -INFINITY, 0.f, -INFINITY);
-                }
-                if (w == 0) s_vr[i % kT8Ring].x = vr;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(B(SC_FULL + i % kT8Ring));
+        } else {
+            uint4 xk[PASSES], xv[PASSES];
+            int p0 = -1, p1 = -1;
+            if (steps > 0) { p0 = page_of(0, 0); p1 = page_of(0, 1); fetch(p0, p1, 0, xk); }
+            for (int i = 0; i < steps && ok; ++i) {
+                fetch(p0, p1, 1, xv);
+                const bool more = i + 1 < steps;
+                if (more) { p0 = page_of(i + 1, 0); p1 = page_of(i + 1, 1); }
+                ok = freed(K_FREE, i);
+                if (!ok) break;
+                widen(sK + (i & 1) * TILE, xk, K_FULL + (i & 1));
+                if (more) fetch(p0, p1, 0, xk);
+                ok = freed(V_FREE, i);
+                if (!ok) break;
+                widen(sV + (i & 1) * TILE, xv, V_FULL + (i & 1));
             }
-            widen(sK + s * TILE, xk);
-            if (lane == 0) mbar_arrive(B(K_FULL + s));
-            p0 = q0; p1 = q1;
-            if (i + 1 < steps) fetch(p0, p1, 0, xk);
-            if (i >= 2) ok = wait8(B(V_FREE + s), ((i >> 1) - 1) & 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            widen(sV + s * TILE, xv);
-            if (lane == 0) mbar_arrive(B(V_FULL + s));
         }
     } else {
         // ---- softmax: thread = query row = TMEM lane ----
+        if constexpr (NT == 2) more_registers<144>(); else more_registers<136>();
+        // this thread's row: q as fp16, K-major with the 128-byte swizzle; rows of no token are zero
+        const int tile = warp >> 2, r = tid & 127;
+        int pos = 0, row_tok = -1, row_head = 0;
+        float row_f = 0.f;
+        {
+            const int rt = tile * toks + r / group;
+            const bool valid = r / group < toks && rt < n;
+            if (valid) { row_tok = t0 + rt; row_head = head * group + r % group; }
+            pos = valid ? min(a.tok_pos[row_tok], most) : -1;
+            uint4 raw[HD / 8];
+            const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + (valid ? (long long)row_tok * a.q_stride + row_head * HD : 0);
+            unsigned top = 0;
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+                raw[c] = make_uint4(0u, 0u, 0u, 0u);
+                if (valid) {
+                    if (a.wide) raw[c] = *reinterpret_cast<const uint4*>(src + 8 * c);
+                    else {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            w[j] = (uint32_t)__bfloat16_as_ushort(src[8 * c + 2 * j]) | (uint32_t)__bfloat16_as_ushort(src[8 * c + 2 * j + 1]) << 16;
+                        raw[c] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[c]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) top = max(top, max((w[j] & 0x7fffu) << 16, w[j] & 0x7fff0000u));
+            }
+            // f = 2^-e with the largest value in [2^(e-1), 2^e), as in the general kernel
+            const int e = min(max((int)(top >> 23) - 126, -125), 125);
+            const float f = top ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
+            row_f = top ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
+            const float fs = a.scale < 0.f ? -f : f;              // block factors are positive: a maximum may be taken before them
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+                float x[8];
+                unpack16<__nv_bfloat16>(raw[c], x);
+                *reinterpret_cast<uint4*>(sQ + tile * TILE + (c >> 3) * HALF + sw128(r, c & 7)) =
+                    make_uint4(pack_half(x[0] * fs, x[1] * fs), pack_half(x[2] * fs, x[3] * fs), pack_half(x[4] * fs, x[5] * fs), pack_half(x[6] * fs, x[7] * fs));
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(B(Q_FULL));
+        }
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t s_at = lanes + tile * kT8Keys, o_at = lanes + NT * kT8Keys + tile * HD;
         const int my_steps = tile ? n1 : n0;
@@ -379,20 +437,44 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT, WW>(), NT == 1 ? 2 : 1) k
                     for (int j = 0; j < 64; ++j)
                         if (k0 + j > open) sv[j] = 0xff800000u;
                 }
-                float mx = -INFINITY;
+                // Weights against the m there is, beside their maximum: the exponentials need not wait for it.  Where a row has passed
+                // m by too much (in its first step, and rarely later), m moves and the weights are computed once more.
+                float l_add;
+                for (;;) {
+                    const float m_use = m == -INFINITY ? 0.f : m;
+                    float mx = -INFINITY;
+                    l_add = 0.f;
+                    uint32_t pk[16];
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    float t4[2] = {__uint_as_float(sv[b * 16]), __uint_as_float(sv[b * 16 + 1])};
+                    for (int b = 0; b < 4; ++b) {
+                        const float4 f = blk[h * 4 + b];
+                        const float c = f.x * row_f, d = f.y - m_use;
+                        float t4[2] = {__uint_as_float(sv[b * 16]), __uint_as_float(sv[b * 16 + 1])};
 #pragma unroll
-                    for (int j = 2; j < 16; j += 4) {
-                        t4[0] = fmaxf(fmaxf(t4[0], __uint_as_float(sv[b * 16 + j])), __uint_as_float(sv[b * 16 + j + 1]));
-                        if (j + 2 < 16) t4[1] = fmaxf(fmaxf(t4[1], __uint_as_float(sv[b * 16 + j + 2])), __uint_as_float(sv[b * 16 + j + 3]));
+                        for (int j = 2; j < 16; j += 4) {
+                            t4[0] = fmaxf(fmaxf(t4[0], __uint_as_float(sv[b * 16 + j])), __uint_as_float(sv[b * 16 + j + 1]));
+                            if (j + 2 < 16) t4[1] = fmaxf(fmaxf(t4[1], __uint_as_float(sv[b * 16 + j + 2])), __uint_as_float(sv[b * 16 + j + 3]));
+                        }
+                        mx = fmaxf(mx, fmaf(fmaxf(t4[0], t4[1]), c, f.w));
+                        const unsigned long long c2 = pair2(c, c), d2 = pair2(d, d);
+                        unsigned long long sum = 0;
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            const float2 x = unpair2(fma2(pair2(__uint_as_float(sv[b * 16 + j]), __uint_as_float(sv[b * 16 + j + 1])), c2, d2));
+                            float w0 = exp2_fast(x.x), w1 = exp2_fast(x.y);
+                            if (MASKED) {                      // also where a factor is NaN
+                                if (k0 + b * 16 + j > open) w0 = 0.f;
+                                if (k0 + b * 16 + j + 1 > open) w1 = 0.f;
+                            }
+                            sum = add2(sum, pair2(w0, w1));
+                            pk[(b & 1) * 8 + j / 2] = pack_half(w0, w1);
+                        }
+                        const float2 s2 = unpair2(sum);
+                        l_add = fmaf(s2.x + s2.y, f.z, l_add);
+                        if (b & 1) tc_st16(s_at + h * 32 + (b >> 1) * 16, pk);       // over columns of S that this thread has read
                     }
-                    const float4 f = blk[h * 4 + b];
-                    mx = fmaxf(mx, fmaf(fmaxf(t4[0], t4[1]), f.x * row_f, f.w));
-                }
-                const bool moves = mx > m + kT8Slack || (m == -INFINITY && mx > m);
-                if (__any_sync(0xffffffffu, moves || vr_now != vr)) {
+                    const bool moves = mx > m + kT8Slack || (m == -INFINITY && mx > m);
+                    if (!__any_sync(0xffffffffu, moves || vr_now != vr)) break;
                     const float m_new = moves ? mx : m;
                     const float corr = m == -INFINITY ? 0.f : exp2_fast(m - m_new);
                     l *= corr;
@@ -423,30 +505,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT, WW>(), NT == 1 ? 2 : 1) k
                     m = m_new;
                     vr = vr_now;
                 }
-                const float m_use = m == -INFINITY ? 0.f : m;
-                uint32_t pk[32];
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const float4 f = blk[h * 4 + b];
-                    const float c = f.x * row_f, d = f.y - m_use;
-                    const unsigned long long c2 = pair2(c, c), d2 = pair2(d, d);
-                    unsigned long long sum = 0;
-#pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        const float2 x = unpair2(fma2(pair2(__uint_as_float(sv[b * 16 + j]), __uint_as_float(sv[b * 16 + j + 1])), c2, d2));
-                        float w0 = exp2_fast(x.x), w1 = exp2_fast(x.y);
-                        if (MASKED) {                          // also where a factor is NaN
-                            if (k0 + b * 16 + j > open) w0 = 0.f;
-                            if (k0 + b * 16 + j + 1 > open) w1 = 0.f;
-                        }
-                        sum = add2(sum, pair2(w0, w1));
-                        pk[b * 8 + j / 2] = pack_half(w0, w1);
-                    }
-                    const float2 s2 = unpair2(sum);
-                    l = fmaf(s2.x + s2.y, f.z, l);
-                }
-                tc_st16(s_at + h * 32, pk);                    // over columns of S that this thread has read
-                tc_st16(s_at + h * 32 + 16, pk + 16);
+                l += l_add;
             }
         };
         for (int i = 0; i < my_steps && ok; ++i) {
@@ -484,7 +543,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT, WW>(), NT == 1 ? 2 : 1) k
     if (!ok && a.status) atomicExch(a.status, 5);
     tc_fence_before();
     __syncthreads();
-    if (warp == SOFT + WW) {
+    if (warp == SOFT + WIDE) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
     }

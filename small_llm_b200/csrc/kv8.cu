@@ -205,12 +205,12 @@ int attn_hd(const Plan& p, int dev, void* stream) {
     const long long pairs = (long long)a.n_tok * a.n_heads;
     return launch(what, k_attn_kv8_join<T, HD>, dim3((unsigned)((pairs + 3) / 4)), 128, 0, stream, a);
 }
-template <int HD, int NT, int WW>
+template <int HD, int NT>
 int attn_tc(const Plan& p, int dev, void* stream) {
     static std::atomic<uint64_t> done{0};
     const char* what = "sllm_k_attn_kv8";
-    if (int rc = opt_in(what, k_attn_kv8_tc<HD, NT, WW>, attn8_tc_smem<HD, NT>(), dev, done)) return rc;
-    return launch(what, k_attn_kv8_tc<HD, NT, WW>, dim3(p.a.c.H, p.tiles), attn8_tc_threads<NT, WW>(), attn8_tc_smem<HD, NT>(), stream, p.a);
+    if (int rc = opt_in(what, k_attn_kv8_tc<HD, NT>, attn8_tc_smem<HD, NT>(), dev, done)) return rc;
+    return launch(what, k_attn_kv8_tc<HD, NT>, dim3(p.a.c.H, p.tiles), attn8_tc_threads<NT>(), attn8_tc_smem<HD, NT>(), stream, p.a);
 }
 template <typename T>
 int attn_t(const Plan& p, uint32_t hd, int dev, void* stream) {
@@ -296,7 +296,7 @@ int sllm_k_attn_kv8(const sllm_kv8_layer* c, const sllm_kv8_attn* s, void* works
         p.a.part = static_cast<float*>(workspace);
         p.a.part_ml = p.a.part + (size_t)p.a.n_tok * p.a.n_heads * p.a.n_chunks * c->head_dim;
     }
-    if (p.tc) return c->head_dim == 64 ? attn_tc<64, 1, 2>(p, dev, stream) : attn_tc<128, 2, 4>(p, dev, stream);
+    if (p.tc) return c->head_dim == 64 ? attn_tc<64, 1>(p, dev, stream) : attn_tc<128, 2>(p, dev, stream);
     return s->dtype == SLLM_ROWS_F32 ? attn_t<float>(p, c->head_dim, dev, stream) : attn_t<__nv_bfloat16>(p, c->head_dim, dev, stream);
 }
 
