@@ -25,9 +25,10 @@
 namespace sllm {
 
 constexpr int kT8Rows = 128;                     // query rows of a tile
-constexpr int kT8Keys = 128;                     // keys of a step
+constexpr int kT8Keys = kPage;                   // keys of a step: a page
 constexpr int kT8Blks = kT8Keys / kBlk8;         // scale blocks of a step
-constexpr int kT8Ring = 4;                       // steps whose scales are held
+constexpr int kT8Ring = 8;                       // steps whose scales are held
+constexpr int kT8Stages = 3;                     // widened K (and V) tiles
 constexpr float kT8Slack = 8.f;                  // log2 units that scores may pass m by
 constexpr int kT8MaxSort = 256;                  // sequences up to which blocks order the tiles by their keys
 
@@ -37,7 +38,7 @@ constexpr int kT8MaxSort = 256;                  // sequences up to which blocks
 // widening 256 x 72 (128 x 64) and the last four warps 128 x 48 (128 x 40): 61440 (30720).
 template <int NT> __host__ __device__ constexpr int attn8_tc_threads() { return NT == 2 ? 640 : 384; }
 template <int HD, int NT> __host__ __device__ constexpr size_t attn8_tc_smem() {
-    return 1024 + NT * (size_t)kT8Rows * HD * 2 + 4 * (size_t)kT8Keys * HD * 2 + kT8Ring * (kT8Blks + 1) * 16 + 256;
+    return 1024 + NT * (size_t)kT8Rows * HD * 2 + 2 * kT8Stages * (size_t)kT8Keys * HD * 2 + kT8Ring * (kT8Blks + 1) * 16 + 256;
 }
 
 __device__ __forceinline__ bool wait8(uint32_t bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, kWaitLimitNs); }
@@ -112,22 +113,24 @@ template <int HD, int NT>
 __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_attn_kv8_tc(const Attn8Args a) {
     constexpr int SOFT = 4 * NT, WIDE = 4 * NT;               // softmax warps 0 .. SOFT - 1, then the widening ones, MMA, scales
     constexpr int THREADS = attn8_tc_threads<NT>();
-    constexpr uint32_t TMEM_COLS = NT * (kT8Keys + HD) > 256 ? 512 : 256;
+    constexpr uint32_t TMEM_COLS = NT * (2 * kT8Keys + HD) > 256 ? 512 : 256;      // two S per tile, and O
     constexpr int HALVES = HD / 64;                           // 128-byte column blocks of a row
-    constexpr uint32_t HALF = kT8Keys * 128;                  // bytes of one of them (query rows and keys are both 128)
-    constexpr uint32_t TILE = HALVES * HALF;
+    constexpr uint32_t Q_HALF = kT8Rows * 128, HALF = kT8Keys * 128;       // bytes of one of them, of queries and of keys
+    constexpr uint32_t Q_TILE = HALVES * Q_HALF, TILE = HALVES * HALF;
     constexpr int CPR = HD / 16;                              // 16-byte chunks of int8 per cache row
     constexpr int RPP = 128 / CPR;              // rows per pass of the widening threads
     constexpr int PASSES = kT8Keys / RPP;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t* sQ = smem;                                       // [2][TILE]
-    uint8_t* sK = sQ + NT * TILE;                              // [2 stages][TILE]
-    uint8_t* sV = sK + 2 * TILE;
-    float4* s_blk = reinterpret_cast<float4*>(sV + 2 * TILE); // [ring][blocks]: c, log2 v, 1 / v, 0 or -inf (blocks that do not count)
+    uint8_t* sQ = smem;                                       // [NT][Q_TILE]
+    uint8_t* sK = sQ + NT * Q_TILE;                           // [stages][TILE]
+    uint8_t* sV = sK + kT8Stages * TILE;
+    float4* s_blk = reinterpret_cast<float4*>(sV + kT8Stages * TILE);      // [ring][blocks]: c, log2 v, 1 / v, 0 or -inf (blocks that do not count)
     float4* s_vr = s_blk + kT8Ring * kT8Blks;                 // [ring]: vr
     uint64_t* bars = reinterpret_cast<uint64_t*>(s_vr + kT8Ring);
-    enum { K_FULL = 0, V_FULL = 2, K_FREE = 4, V_FREE = 6, S_READY = 8, P_READY = 10, SC_FULL = 12, O_DONE = 16, Q_FULL = 17, N_BARS = 18 };
+    // S_READY, P_READY and PV_DONE: [tile][step parity], for they may be a step ahead of who waits
+    enum { K_FULL = 0, V_FULL = K_FULL + kT8Stages, K_FREE = V_FULL + kT8Stages, V_FREE = K_FREE + kT8Stages, S_READY = V_FREE + kT8Stages, P_READY = S_READY + 4,
+           PV_DONE = P_READY + 4, SC_FULL = PV_DONE + 4, Q_FULL = SC_FULL + kT8Ring, N_BARS = Q_FULL + 1 };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
     __shared__ int s_last[2][8];
     __shared__ int s_len[kT8MaxSort], s_tiles[kT8MaxSort], s_pick[2];
@@ -169,13 +172,10 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
     const int most = (int)min((long long)a.width * kPage, 0x7fffff00ll) - 1;
 
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(B(K_FULL + i), 4); mbar_init(B(V_FULL + i), 4);
-            mbar_init(B(K_FREE + i), 1); mbar_init(B(V_FREE + i), 1);
-            mbar_init(B(S_READY + i), 1); mbar_init(B(P_READY + i), 4);
-        }
+        for (int i = 0; i < kT8Stages; ++i) { mbar_init(B(K_FULL + i), 4); mbar_init(B(V_FULL + i), 4); mbar_init(B(K_FREE + i), 1); mbar_init(B(V_FREE + i), 1); }
+        for (int i = 0; i < 4; ++i) { mbar_init(B(S_READY + i), 1); mbar_init(B(P_READY + i), 4); mbar_init(B(PV_DONE + i), 1); }
         for (int i = 0; i < kT8Ring; ++i) mbar_init(B(SC_FULL + i), 1);
-        mbar_init(B(O_DONE), 1); mbar_init(B(Q_FULL), SOFT);
+        mbar_init(B(Q_FULL), SOFT);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == SOFT + WIDE) {
@@ -201,12 +201,11 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
     bool ok = true;
 
     const int* table = a.table + (size_t)seq * a.width;
-    auto page_of = [&](int i, int half) -> int {              // page of a step's first or second 64 keys; -1: behind the last position, -2: outside the pool
-        const int p = 2 * i + half;
-        if ((long long)p * kPage > last) return -1;
-        const int id = table[p];
+    auto page_of = [&](int i) -> int {                        // page of a step; -2: outside the pool
+        const int id = table[i];
         return id < 0 || id >= a.c.n_pages ? -2 : id;
     };
+    auto parity = [](int i) { return (uint32_t)(i / kT8Stages) & 1u; };       // of step i's use of its stage
     if (warp >= SOFT + WIDE) {
         fewer_registers<NT == 2 ? 48 : 40>();
         if (warp == SOFT + WIDE) {
@@ -216,77 +215,78 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
         // descriptors of the first tiles; a place further on is its distance / 16 more
         const uint32_t q_desc = desc_lo(sQ), k_desc = desc_lo(sK), v_desc = desc_lo(sV);
         auto issue_s = [&](int i, int t) {
-            const uint32_t q = q_desc + (uint32_t)t * (TILE / 16), k = k_desc + (uint32_t)(i & 1) * (TILE / 16);
+            const uint32_t q = q_desc + (uint32_t)t * (Q_TILE / 16), k = k_desc + (uint32_t)(i % kT8Stages) * (TILE / 16);
+            const uint32_t d = tmem + (uint32_t)((2 * t + (i & 1)) * kT8Keys);
             if (elect_one()) {
 #pragma unroll
-                for (int j = 0; j < HD / 16; ++j) {
-                    const uint32_t at = ((j >> 2) * HALF + (j & 3) * 32) / 16;
-                    tc_mma_f16_ss(tmem + (uint32_t)(t * kT8Keys), q + at, k + at, id_s, j != 0);
-                }
-                tc_commit(B(S_READY + t));
+                for (int j = 0; j < HD / 16; ++j)
+                    tc_mma_f16_ss(d, q + ((j >> 2) * Q_HALF + (j & 3) * 32) / 16, k + ((j >> 2) * HALF + (j & 3) * 32) / 16, id_s, j != 0);
+                tc_commit(B(S_READY + 2 * t + (i & 1)));
             }
             __syncwarp();
         };
         auto issue_o = [&](int i, int t) {
-            const uint32_t v = v_desc + (uint32_t)(i & 1) * (TILE / 16);
+            const uint32_t v = v_desc + (uint32_t)(i % kT8Stages) * (TILE / 16), p = tmem + (uint32_t)((2 * t + (i & 1)) * kT8Keys);
             if (elect_one()) {
 #pragma unroll
                 for (int h = 0; h < HALVES; ++h)
 #pragma unroll
                     for (int j = 0; j < kT8Keys / 16; ++j)
-                        tc_mma_f16_ts(tmem + NT * kT8Keys + t * HD + h * 64, tmem + (uint32_t)(t * kT8Keys + j * 8), v + (h * HALF + j * 2048) / 16, id_o, i > 0 || j > 0);
+                        tc_mma_f16_ts(tmem + NT * 2 * kT8Keys + t * HD + h * 64, p + j * 8, v + (h * HALF + j * 2048) / 16, id_o, i > 0 || j > 0);
+                tc_commit(B(PV_DONE + 2 * t + (i & 1)));
             }
             __syncwarp();
         };
         auto commit = [&](int bar) { if (elect_one()) tc_commit(B(bar)); __syncwarp(); };
         // A wait that gives up does so in every lane or soon after: the warp goes on as one.
-        auto wait = [&](int bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, wait8(B(bar), parity)); };
-        if (steps > 0) {
-            ok = wait(Q_FULL, 0) && wait(K_FULL, 0);
+        auto wait = [&](int bar, uint32_t par) { return (bool)__all_sync(0xffffffffu, wait8(B(bar), par)); };
+        // S runs two steps ahead of the softmax: it has the next step's scores when it ends one
+        if (steps > 0) ok = wait(Q_FULL, 0);
+        for (int i = 0; i < 2 && i < steps && ok; ++i) {
+            ok = wait(K_FULL + i, 0) && wait(SC_FULL + i, 0);
             tc_fence_after();
-            if (ok && n0 > 0) issue_s(0, 0);
-            if (ok && n1 > 0) issue_s(0, 1);
-            if (ok) commit(K_FREE);
+            for (int t = 0; t < NT; ++t)
+                if (ok && i < (t ? n1 : n0)) issue_s(i, t);
+            if (ok) commit(K_FREE + i);
         }
         for (int i = 0; i < steps && ok; ++i) {
-            const int s = i & 1;
-            ok = wait(V_FULL + s, (i >> 1) & 1);
+            ok = wait(V_FULL + i % kT8Stages, parity(i));
             for (int t = 0; t < NT && ok; ++t) {
                 const int nt = t ? n1 : n0;
                 if (i < nt) {
-                    ok = wait(P_READY + t, i & 1);
+                    ok = wait(P_READY + 2 * t + (i & 1), (i >> 1) & 1);
                     if (!ok) break;
                     tc_fence_after();
                     issue_o(i, t);
                 }
-                if (i + 1 < nt) {
-                    ok = wait(K_FULL + (s ^ 1), ((i + 1) >> 1) & 1);
+                if (i + 2 < nt) {
+                    // the scales too, though S does not need them: their warp then has never more than one phase of K_FREE to catch up with
+                    ok = wait(K_FULL + (i + 2) % kT8Stages, parity(i + 2)) && wait(SC_FULL + (i + 2) % kT8Ring, ((i + 2) / kT8Ring) & 1);
                     if (!ok) break;
                     tc_fence_after();
-                    issue_s(i + 1, t);
+                    issue_s(i + 2, t);
                 }
             }
             if (!ok) break;
-            commit(V_FREE + s);
-            if (i + 1 < steps) commit(K_FREE + (s ^ 1));
+            commit(V_FREE + i % kT8Stages);
+            if (i + 2 < steps) commit(K_FREE + (i + 2) % kT8Stages);
         }
-        if (ok && steps > 0) commit(O_DONE);
         } else if (warp == SOFT + WIDE + 1) {
         // ---- the blocks' factors: lane b takes block b of a step; the loads are a step ahead ----
         float ks = 0.f, vs = 0.f, vr = 0.f;
         bool counts = false;
-        int id = lane < kT8Blks && steps > 0 ? page_of(0, lane / kBlksPerPage) : -1;
+        int id = lane < kT8Blks && steps > 0 ? page_of(0) : -1;
         auto fetch = [&](int i) {
             counts = id >= 0 && (long long)i * kT8Keys + lane * kBlk8 <= last;
             if (id == -2 && a.status) atomicExch(a.status, 1);
             if (counts) {
-                const float* sc = a.c.scales + ((long long)id * a.c.H + head) * 2 * kBlksPerPage + (lane % kBlksPerPage);
+                const float* sc = a.c.scales + ((long long)id * a.c.H + head) * 2 * kBlksPerPage + lane;
                 ks = sc[0]; vs = sc[kBlksPerPage];
             }
         };
         if (steps > 0) fetch(0);
         for (int i = 0; i < steps && ok; ++i) {
-            id = lane < kT8Blks && i + 1 < steps ? page_of(i + 1, lane / kBlksPerPage) : -1;
+            id = lane < kT8Blks && i + 1 < steps ? page_of(i + 1) : -1;
             float top = counts && vs == vs ? vs : 0.f;
 #pragma unroll
             for (int o = 1; o < kT8Blks; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -294,8 +294,9 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
             const float v0 = vr > 0.f ? vs / vr : (vs == 0.f ? 1.f : vs);
             const float v = v0 != v0 ? v0 : fmaxf(v0, 8.67361738e-19f);              // 2^-60: fp16 takes such a weight for 0, the sum does not
             const float4 f = counts ? make_float4(ks * fabsf(a.scale) * 1.4426950408889634f, log2f(v), 1.f / v, 0.f) : make_float4(0.f, -INFINITY, 0.f, -INFINITY);
-            // step i - 2's K is free: the softmax is done with step i - 3, whose place in the ring may be written
-            if (i >= 2) ok = __all_sync(0xffffffffu, wait8(B(K_FREE + (i & 1)), ((i >> 1) - 1) & 1));
+            // the K of a step is free once S is done, which was asked for when the softmax had ended the step two before: with the
+            // K of step i - stages free it is done with i - stages - 2, far behind the ring's length
+            if (i >= kT8Stages) ok = __all_sync(0xffffffffu, wait8(B(K_FREE + i % kT8Stages), parity(i - kT8Stages)));
             if (!ok) break;
             if (lane < kT8Blks) s_blk[(i % kT8Ring) * kT8Blks + lane] = f;
             if (lane == 0) s_vr[i % kT8Ring].x = vr;
@@ -312,15 +313,10 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
         // the two column blocks of head_dim 128 store the halves of a chunk in opposite order: no bank conflicts
         const int swap = HALVES == 2 ? (c >> 2) & 1 : 0, ch = (2 * c) & 7;
         const uint32_t at0 = (c >> 2) * HALF + sw128(row0, ch + swap), at1 = (c >> 2) * HALF + sw128(row0, ch + 1 - swap);
-        auto fetch = [&](int p0, int p1, int which, uint4 (&x)[PASSES]) {
+        auto fetch = [&](int id, int which, uint4 (&x)[PASSES]) {
+            const int8_t* src = a.c.pages + (((long long)id * a.c.H + head) * 2 + which) * (kPage * HD) + row0 * HD + c * 16;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int id = h ? p1 : p0;
-                const int8_t* src = a.c.pages + (((long long)id * a.c.H + head) * 2 + which) * (kPage * HD) + row0 * HD + c * 16;
-#pragma unroll
-                for (int j = 0; j < PASSES / 2; ++j)
-                    x[h * (PASSES / 2) + j] = id >= 0 ? *reinterpret_cast<const uint4*>(src + j * RPP * HD) : make_uint4(0u, 0u, 0u, 0u);
-            }
+            for (int j = 0; j < PASSES; ++j) x[j] = id >= 0 ? *reinterpret_cast<const uint4*>(src + j * RPP * HD) : make_uint4(0u, 0u, 0u, 0u);
         };
         auto widen = [&](uint8_t* dst, const uint4 (&x)[PASSES], int full) {
 #pragma unroll
@@ -335,37 +331,37 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
             __syncwarp();
             if (lane == 0) mbar_arrive(B(full));
         };
-        auto freed = [&](int bar, int i) { return i < 2 || __all_sync(0xffffffffu, wait8(B(bar + (i & 1)), ((i >> 1) - 1) & 1)); };
+        auto freed = [&](int bar, int i) { return i < kT8Stages || __all_sync(0xffffffffu, wait8(B(bar + i % kT8Stages), parity(i - kT8Stages))); };
         if constexpr (NT == 2) {
             const int which = (warp - SOFT) >> 2;
             uint8_t* dst = which ? sV : sK;
             const int full = which ? V_FULL : K_FULL, free = which ? V_FREE : K_FREE;
             uint4 x[PASSES];
-            int p0 = -1, p1 = -1;
-            if (steps > 0) { p0 = page_of(0, 0); p1 = page_of(0, 1); fetch(p0, p1, which, x); }
+            int id = -1;
+            if (steps > 0) fetch(page_of(0), which, x);
+            if (steps > 1) id = page_of(1);
             for (int i = 0; i < steps && ok; ++i) {
-                const bool more = i + 1 < steps;
-                if (more) { p0 = page_of(i + 1, 0); p1 = page_of(i + 1, 1); }
                 ok = freed(free, i);
                 if (!ok) break;
-                widen(dst + (i & 1) * TILE, x, full + (i & 1));
-                if (more) fetch(p0, p1, which, x);
+                widen(dst + (i % kT8Stages) * TILE, x, full + i % kT8Stages);
+                if (i + 1 < steps) fetch(id, which, x);
+                if (i + 2 < steps) id = page_of(i + 2);
             }
         } else {
             uint4 xk[PASSES], xv[PASSES];
-            int p0 = -1, p1 = -1;
-            if (steps > 0) { p0 = page_of(0, 0); p1 = page_of(0, 1); fetch(p0, p1, 0, xk); }
+            int id = -1;
+            if (steps > 0) { id = page_of(0); fetch(id, 0, xk); fetch(id, 1, xv); }
+            if (steps > 1) id = page_of(1);
             for (int i = 0; i < steps && ok; ++i) {
-                fetch(p0, p1, 1, xv);
-                const bool more = i + 1 < steps;
-                if (more) { p0 = page_of(i + 1, 0); p1 = page_of(i + 1, 1); }
                 ok = freed(K_FREE, i);
                 if (!ok) break;
-                widen(sK + (i & 1) * TILE, xk, K_FULL + (i & 1));
-                if (more) fetch(p0, p1, 0, xk);
+                widen(sK + (i % kT8Stages) * TILE, xk, K_FULL + i % kT8Stages);
+                if (i + 1 < steps) fetch(id, 0, xk);
                 ok = freed(V_FREE, i);
                 if (!ok) break;
-                widen(sV + (i & 1) * TILE, xv, V_FULL + (i & 1));
+                widen(sV + (i % kT8Stages) * TILE, xv, V_FULL + i % kT8Stages);
+                if (i + 1 < steps) fetch(id, 1, xv);
+                if (i + 2 < steps) id = page_of(i + 2);
             }
         }
     } else {
@@ -409,7 +405,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
             for (int c = 0; c < HD / 8; ++c) {
                 float x[8];
                 unpack16<__nv_bfloat16>(raw[c], x);
-                *reinterpret_cast<uint4*>(sQ + tile * TILE + (c >> 3) * HALF + sw128(r, c & 7)) =
+                *reinterpret_cast<uint4*>(sQ + tile * Q_TILE + (c >> 3) * Q_HALF + sw128(r, c & 7)) =
                     make_uint4(pack_half(x[0] * fs, x[1] * fs), pack_half(x[2] * fs, x[3] * fs), pack_half(x[4] * fs, x[5] * fs), pack_half(x[6] * fs, x[7] * fs));
             }
             fence_async_smem();
@@ -417,113 +413,100 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
             if (lane == 0) mbar_arrive(B(Q_FULL));
         }
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t s_at = lanes + tile * kT8Keys, o_at = lanes + NT * kT8Keys + tile * HD;
+        const uint32_t o_at = lanes + NT * 2 * kT8Keys + tile * HD;
         const int my_steps = tile ? n1 : n0;
         const int open = row_tok >= 0 ? pos : 0x7fffffff;      // rows of no token: q = 0, whatever they come to is not written
         const int all_see = __reduce_min_sync(0xffffffffu, open);
         float m = -INFINITY, l = 0.f, vr = 0.f;
-        // One step, 64 keys at a time so that their scores stay in registers: maximum, weights, and the weights over the scores.
-        auto half_steps = [&](auto masked, const float4* blk, float vr_now, int kb, bool have_o) {
+        // One step: the 64 scores of a row stay in registers.
+        auto step = [&](auto masked, int i) {
             constexpr bool MASKED = decltype(masked)::value;
-#pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
-                uint32_t sv[64];
-                tc_ld32_async(s_at + h * 64, sv);
-                tc_ld32_async(s_at + h * 64 + 32, sv + 32);
-                tc_wait_ld64(sv);
-                const int k0 = kb + h * 64;
-                if (MASKED) {
+            const float4* blk = s_blk + (i % kT8Ring) * kT8Blks;
+            const float vr_now = s_vr[i % kT8Ring].x;
+            const uint32_t s_at = lanes + (uint32_t)((2 * tile + (i & 1)) * kT8Keys);
+            const int k0 = i * kT8Keys;
+            uint32_t sv[64];
+            tc_ld32_async(s_at, sv);
+            tc_ld32_async(s_at + 32, sv + 32);
+            tc_wait_ld64(sv);
+            if (MASKED) {
 #pragma unroll
-                    for (int j = 0; j < 64; ++j)
-                        if (k0 + j > open) sv[j] = 0xff800000u;
-                }
-                // Weights against the m there is, beside their maximum: the exponentials need not wait for it.  Where a row has passed
-                // m by too much (in its first step, and rarely later), m moves and the weights are computed once more.
-                float l_add;
-                for (;;) {
-                    const float m_use = m == -INFINITY ? 0.f : m;
-                    float mx = -INFINITY;
-                    l_add = 0.f;
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const float4 f = blk[h * 4 + b];
-                        const float c = f.x * row_f, d = f.y - m_use;
-                        float t4[2] = {__uint_as_float(sv[b * 16]), __uint_as_float(sv[b * 16 + 1])};
-#pragma unroll
-                        for (int j = 2; j < 16; j += 4) {
-                            t4[0] = fmaxf(fmaxf(t4[0], __uint_as_float(sv[b * 16 + j])), __uint_as_float(sv[b * 16 + j + 1]));
-                            if (j + 2 < 16) t4[1] = fmaxf(fmaxf(t4[1], __uint_as_float(sv[b * 16 + j + 2])), __uint_as_float(sv[b * 16 + j + 3]));
-                        }
-                        mx = fmaxf(mx, fmaf(fmaxf(t4[0], t4[1]), c, f.w));
-                        const unsigned long long c2 = pair2(c, c), d2 = pair2(d, d);
-                        unsigned long long sum = 0;
-#pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            const float2 x = unpair2(fma2(pair2(__uint_as_float(sv[b * 16 + j]), __uint_as_float(sv[b * 16 + j + 1])), c2, d2));
-                            float w0 = exp2_fast(x.x), w1 = exp2_fast(x.y);
-                            if (MASKED) {                      // also where a factor is NaN
-                                if (k0 + b * 16 + j > open) w0 = 0.f;
-                                if (k0 + b * 16 + j + 1 > open) w1 = 0.f;
-                            }
-                            sum = add2(sum, pair2(w0, w1));
-                            pk[(b & 1) * 8 + j / 2] = pack_half(w0, w1);
-                        }
-                        const float2 s2 = unpair2(sum);
-                        l_add = fmaf(s2.x + s2.y, f.z, l_add);
-                        if (b & 1) tc_st16(s_at + h * 32 + (b >> 1) * 16, pk);       // over columns of S that this thread has read
-                    }
-                    const bool moves = mx > m + kT8Slack || (m == -INFINITY && mx > m);
-                    if (!__any_sync(0xffffffffu, moves || vr_now != vr)) break;
-                    const float m_new = moves ? mx : m;
-                    const float corr = m == -INFINITY ? 0.f : exp2_fast(m - m_new);
-                    l *= corr;
-                    uint32_t x[16];
-                    if (have_o) {                              // every product into O so far is done: S of this step came after them
-                        const float f = corr * (vr_now > 0.f ? vr / vr_now : 1.f);
-#pragma unroll 1
-                        for (int c = 0; c < HD / 16; ++c) {
-                            tc_ld16(o_at + c * 16, x);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * f);
-                            tc_st16(o_at + c * 16, x);
-                        }
-                    }
-                    if (h == 1) {                              // the weights of this step's first half are relative to the old m
-                        tc_wait_st();
-#pragma unroll 1
-                        for (int c = 0; c < 2; ++c) {
-                            tc_ld16(s_at + c * 16, x);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&x[j]));
-                                x[j] = pack_half(w.x * corr, w.y * corr);
-                            }
-                            tc_st16(s_at + c * 16, x);
-                        }
-                    }
-                    m = m_new;
-                    vr = vr_now;
-                }
-                l += l_add;
+                for (int j = 0; j < 64; ++j)
+                    if (k0 + j > open) sv[j] = 0xff800000u;
             }
+            // Weights against the m there is, beside their maximum: the exponentials need not wait for it.  Where a row has passed
+            // m by too much (in its first step, and rarely later), m moves and the weights are computed once more.
+            float l_add;
+            for (;;) {
+                const float m_use = m == -INFINITY ? 0.f : m;
+                float mx = -INFINITY;
+                l_add = 0.f;
+                uint32_t pk[16];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const float4 f = blk[b];
+                    const float c = f.x * row_f, d = f.y - m_use;
+                    float t4[2] = {__uint_as_float(sv[b * 16]), __uint_as_float(sv[b * 16 + 1])};
+#pragma unroll
+                    for (int j = 2; j < 16; j += 4) {
+                        t4[0] = fmaxf(fmaxf(t4[0], __uint_as_float(sv[b * 16 + j])), __uint_as_float(sv[b * 16 + j + 1]));
+                        if (j + 2 < 16) t4[1] = fmaxf(fmaxf(t4[1], __uint_as_float(sv[b * 16 + j + 2])), __uint_as_float(sv[b * 16 + j + 3]));
+                    }
+                    mx = fmaxf(mx, fmaf(fmaxf(t4[0], t4[1]), c, f.w));
+                    const unsigned long long c2 = pair2(c, c), d2 = pair2(d, d);
+                    unsigned long long sum = 0;
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        const float2 x = unpair2(fma2(pair2(__uint_as_float(sv[b * 16 + j]), __uint_as_float(sv[b * 16 + j + 1])), c2, d2));
+                        float w0 = exp2_fast(x.x), w1 = exp2_fast(x.y);
+                        if (MASKED) {                      // also where a factor is NaN
+                            if (k0 + b * 16 + j > open) w0 = 0.f;
+                            if (k0 + b * 16 + j + 1 > open) w1 = 0.f;
+                        }
+                        sum = add2(sum, pair2(w0, w1));
+                        pk[(b & 1) * 8 + j / 2] = pack_half(w0, w1);
+                    }
+                    const float2 s2 = unpair2(sum);
+                    l_add = fmaf(s2.x + s2.y, f.z, l_add);
+                    if (b & 1) tc_st16(s_at + (b >> 1) * 16, pk);       // over columns of S that this thread has read
+                }
+                const bool moves = mx > m + kT8Slack || (m == -INFINITY && mx > m);
+                if (!__any_sync(0xffffffffu, moves || vr_now != vr)) break;
+                const float m_new = moves ? mx : m;
+                const float corr = m == -INFINITY ? 0.f : exp2_fast(m - m_new);
+                l *= corr;
+                uint32_t x[16];
+                if (i > 0) {                               // O is still as the products left it: the last of them has to be done
+                    if (ok) ok = wait8(B(PV_DONE + 2 * tile + ((i - 1) & 1)), ((i - 1) >> 1) & 1);
+                    ok = __all_sync(0xffffffffu, ok);
+                    tc_fence_after();
+                    const float f = corr * (vr_now > 0.f ? vr / vr_now : 1.f);
+#pragma unroll 1
+                    for (int c = 0; c < HD / 16; ++c) {
+                        tc_ld16(o_at + c * 16, x);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * f);
+                        tc_st16(o_at + c * 16, x);
+                    }
+                }
+                m = m_new;
+                vr = vr_now;
+            }
+            l += l_add;
         };
         for (int i = 0; i < my_steps && ok; ++i) {
-            ok = wait8(B(SC_FULL + i % kT8Ring), (i / kT8Ring) & 1) && wait8(B(S_READY + tile), i & 1);
+            ok = wait8(B(SC_FULL + i % kT8Ring), (i / kT8Ring) & 1) && wait8(B(S_READY + 2 * tile + (i & 1)), (i >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            const float4* blk = s_blk + (i % kT8Ring) * kT8Blks;
-            const float vr_now = s_vr[i % kT8Ring].x;
-            const int kb = i * kT8Keys;
-            if (kb + kT8Keys - 1 > all_see) half_steps(std::integral_constant<bool, true>{}, blk, vr_now, kb, i > 0);
-            else half_steps(std::integral_constant<bool, false>{}, blk, vr_now, kb, i > 0);
+            if (i * kT8Keys + kT8Keys - 1 > all_see) step(std::integral_constant<bool, true>{}, i);     // the same for the whole warp
+            else step(std::integral_constant<bool, false>{}, i);
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(B(P_READY + tile));
+            if (lane == 0) mbar_arrive(B(P_READY + 2 * tile + (i & 1)));
         }
-        if (steps > 0 && ok) ok = wait8(B(O_DONE), 0);
+        if (my_steps > 0 && ok) ok = wait8(B(PV_DONE + 2 * tile + ((my_steps - 1) & 1)), ((my_steps - 1) >> 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
         if (ok) {
