@@ -28,7 +28,7 @@ constexpr int kT8Rows = 128;                     // query rows of a tile
 constexpr int kT8Keys = kPage;                   // keys of a step: a page
 constexpr int kT8Blks = kT8Keys / kBlk8;         // scale blocks of a step
 constexpr int kT8Ring = 8;                       // steps whose scales are held
-constexpr int kT8Stages = 3;                     // widened K (and V) tiles
+constexpr int kT8Stages = 4;                     // widened K (and V) tiles
 constexpr float kT8Slack = 8.f;                  // log2 units that scores may pass m by
 constexpr int kT8MaxSort = 256;                  // sequences up to which blocks order the tiles by their keys
 
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
     const int most = (int)min((long long)a.width * kPage, 0x7fffff00ll) - 1;
 
     if (tid == 0) {
-        for (int i = 0; i < kT8Stages; ++i) { mbar_init(B(K_FULL + i), 4); mbar_init(B(V_FULL + i), 4); mbar_init(B(K_FREE + i), 1); mbar_init(B(V_FREE + i), 1); }
+        for (int i = 0; i < kT8Stages; ++i) { mbar_init(B(K_FULL + i), 5); mbar_init(B(V_FULL + i), 4); mbar_init(B(K_FREE + i), 1); mbar_init(B(V_FREE + i), 1); }
         for (int i = 0; i < 4; ++i) { mbar_init(B(S_READY + i), 1); mbar_init(B(P_READY + i), 4); mbar_init(B(PV_DONE + i), 1); }
         for (int i = 0; i < kT8Ring; ++i) mbar_init(B(SC_FULL + i), 1);
         mbar_init(B(Q_FULL), SOFT);
@@ -214,63 +214,59 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
         const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(kT8Rows >> 4) << 24);   // V: MN-major
         // descriptors of the first tiles; a place further on is its distance / 16 more
         const uint32_t q_desc = desc_lo(sQ), k_desc = desc_lo(sK), v_desc = desc_lo(sV);
-        auto issue_s = [&](int i, int t) {
-            const uint32_t q = q_desc + (uint32_t)t * (Q_TILE / 16), k = k_desc + (uint32_t)(i % kT8Stages) * (TILE / 16);
-            const uint32_t d = tmem + (uint32_t)((2 * t + (i & 1)) * kT8Keys);
-            if (elect_one()) {
+        // One lane does it all: as few instructions as can be, for four busy warps share its scheduler.
+        if (elect_one()) {
+            auto issue_s = [&](int i, int t) {
+                const uint32_t q = q_desc + (uint32_t)t * (Q_TILE / 16), k = k_desc + (uint32_t)(i % kT8Stages) * (TILE / 16);
+                const uint32_t d = tmem + (uint32_t)((2 * t + (i & 1)) * kT8Keys);
 #pragma unroll
                 for (int j = 0; j < HD / 16; ++j)
                     tc_mma_f16_ss(d, q + ((j >> 2) * Q_HALF + (j & 3) * 32) / 16, k + ((j >> 2) * HALF + (j & 3) * 32) / 16, id_s, j != 0);
                 tc_commit(B(S_READY + 2 * t + (i & 1)));
-            }
-            __syncwarp();
-        };
-        auto issue_o = [&](int i, int t) {
-            const uint32_t v = v_desc + (uint32_t)(i % kT8Stages) * (TILE / 16), p = tmem + (uint32_t)((2 * t + (i & 1)) * kT8Keys);
-            if (elect_one()) {
+            };
+            auto issue_o = [&](int i, int t) {
+                const uint32_t v = v_desc + (uint32_t)(i % kT8Stages) * (TILE / 16), p = tmem + (uint32_t)((2 * t + (i & 1)) * kT8Keys);
 #pragma unroll
                 for (int h = 0; h < HALVES; ++h)
 #pragma unroll
                     for (int j = 0; j < kT8Keys / 16; ++j)
                         tc_mma_f16_ts(tmem + NT * 2 * kT8Keys + t * HD + h * 64, p + j * 8, v + (h * HALF + j * 2048) / 16, id_o, i > 0 || j > 0);
                 tc_commit(B(PV_DONE + 2 * t + (i & 1)));
+            };
+            // S runs two steps ahead of the softmax: it has the next step's scores when it ends one.  K_FULL stands for the scales
+            // as well, which S does not need: so their warp, which K_FREE holds back, is never a whole phase of it behind.
+            if (steps > 0) ok = wait8(B(Q_FULL), 0);
+            for (int i = 0; i < 2 && i < steps && ok; ++i) {
+                ok = wait8(B(K_FULL + i), 0);
+                if (!ok) break;
+                tc_fence_after();
+                if (i < n0) issue_s(i, 0);
+                if (i < n1) issue_s(i, 1);
+                tc_commit(B(K_FREE + i));
             }
-            __syncwarp();
-        };
-        auto commit = [&](int bar) { if (elect_one()) tc_commit(B(bar)); __syncwarp(); };
-        // A wait that gives up does so in every lane or soon after: the warp goes on as one.
-        auto wait = [&](int bar, uint32_t par) { return (bool)__all_sync(0xffffffffu, wait8(B(bar), par)); };
-        // S runs two steps ahead of the softmax: it has the next step's scores when it ends one
-        if (steps > 0) ok = wait(Q_FULL, 0);
-        for (int i = 0; i < 2 && i < steps && ok; ++i) {
-            ok = wait(K_FULL + i, 0) && wait(SC_FULL + i, 0);
-            tc_fence_after();
-            for (int t = 0; t < NT; ++t)
-                if (ok && i < (t ? n1 : n0)) issue_s(i, t);
-            if (ok) commit(K_FREE + i);
-        }
-        for (int i = 0; i < steps && ok; ++i) {
-            ok = wait(V_FULL + i % kT8Stages, parity(i));
-            for (int t = 0; t < NT && ok; ++t) {
-                const int nt = t ? n1 : n0;
-                if (i < nt) {
-                    ok = wait(P_READY + 2 * t + (i & 1), (i >> 1) & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-                    issue_o(i, t);
+            for (int i = 0; i < steps && ok; ++i) {
+                const int s = i % kT8Stages, s2 = (i + 2) % kT8Stages;
+                ok = wait8(B(V_FULL + s), parity(i));
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const int nt = t ? n1 : n0;
+                    if (ok && i < nt) {
+                        ok = wait8(B(P_READY + 2 * t + (i & 1)), (i >> 1) & 1);
+                        tc_fence_after();
+                        if (ok) issue_o(i, t);
+                    }
+                    if (t == 0 && ok && i + 2 < steps) {
+                        ok = wait8(B(K_FULL + s2), parity(i + 2));
+                        tc_fence_after();
+                    }
+                    if (ok && i + 2 < nt) issue_s(i + 2, t);
                 }
-                if (i + 2 < nt) {
-                    // the scales too, though S does not need them: their warp then has never more than one phase of K_FREE to catch up with
-                    ok = wait(K_FULL + (i + 2) % kT8Stages, parity(i + 2)) && wait(SC_FULL + (i + 2) % kT8Ring, ((i + 2) / kT8Ring) & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-                    issue_s(i + 2, t);
-                }
+                if (!ok) break;
+                tc_commit(B(V_FREE + s));
+                if (i + 2 < steps) tc_commit(B(K_FREE + s2));
             }
-            if (!ok) break;
-            commit(V_FREE + i % kT8Stages);
-            if (i + 2 < steps) commit(K_FREE + (i + 2) % kT8Stages);
         }
+        ok = __all_sync(0xffffffffu, ok);
         } else if (warp == SOFT + WIDE + 1) {
         // ---- the blocks' factors: lane b takes block b of a step; the loads are a step ahead ----
         float ks = 0.f, vs = 0.f, vr = 0.f;
@@ -301,7 +297,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
             if (lane < kT8Blks) s_blk[(i % kT8Ring) * kT8Blks + lane] = f;
             if (lane == 0) s_vr[i % kT8Ring].x = vr;
             __syncwarp();
-            if (lane == 0) mbar_arrive(B(SC_FULL + i % kT8Ring));
+            if (lane == 0) { mbar_arrive(B(SC_FULL + i % kT8Ring)); mbar_arrive(B(K_FULL + i % kT8Stages)); }
             if (i + 1 < steps) fetch(i + 1);
         }
         }
