@@ -17,8 +17,6 @@
 // Bound by the exponentials (16 a clock and SM: 1024 clocks per 128 x 128 tile) and, at head_dim 128, equally by the products.
 // Every wait is bounded; on expiry the block sets *status, frees its tensor memory and returns.
 #pragma once
-#include <type_traits>
-
 #include "attn_kv8.cuh"
 #include "tc_ptx.cuh"
 
@@ -289,7 +287,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
             if (top > vr) vr = pow2_above(fminf(top, 1.7e38f));
             const float v0 = vr > 0.f ? vs / vr : (vs == 0.f ? 1.f : vs);
             const float v = v0 != v0 ? v0 : fmaxf(v0, 8.67361738e-19f);              // 2^-60: fp16 takes such a weight for 0, the sum does not
-            const float4 f = counts ? make_float4(ks * fabsf(a.scale) * 1.4426950408889634f, log2f(v), 1.f / v, 0.f) : make_float4(0.f, -INFINITY, 0.f, -INFINITY);
+            const float4 f = counts ? make_float4(ks * fabsf(a.scale) * 1.4426950408889634f, ks == ks ? log2f(v) : ks, 1.f / v, 0.f) : make_float4(0.f, -INFINITY, 0.f, -INFINITY);
             // the K of a step is free once S is done, which was asked for when the softmax had ended the step two before: with the
             // K of step i - stages free it is done with i - stages - 2, far behind the ring's length
             if (i >= kT8Stages) ok = __all_sync(0xffffffffu, wait8(B(K_FREE + i % kT8Stages), parity(i - kT8Stages)));
@@ -304,11 +302,10 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
     } else if (warp >= SOFT) {
         // ---- widening: int8 rows -> fp16 tiles, the loads a step ahead ----
         if constexpr (NT == 2) fewer_registers<72>(); else fewer_registers<64>();
-        const int w = tid & 127, c = w % CPR, row0 = w / CPR;
+        // A warp takes one 128-byte column block of eight rows: its lanes' stores, two rows of four chunks at a time, meet no bank twice.
+        const int wi = warp & 3, c = (lane & 3) + (HALVES == 2 ? (wi >> 1) * 4 : 0), row0 = (lane >> 2) + (HALVES == 2 ? wi & 1 : wi) * 8;
         static_assert(RPP % 8 == 0, "rows of a thread share their place in the swizzle");
-        // the two column blocks of head_dim 128 store the halves of a chunk in opposite order: no bank conflicts
-        const int swap = HALVES == 2 ? (c >> 2) & 1 : 0, ch = (2 * c) & 7;
-        const uint32_t at0 = (c >> 2) * HALF + sw128(row0, ch + swap), at1 = (c >> 2) * HALF + sw128(row0, ch + 1 - swap);
+        const uint32_t at0 = (c >> 2) * HALF + sw128(row0, (2 * c) & 7), at1 = (c >> 2) * HALF + sw128(row0, ((2 * c) & 7) + 1);
         auto fetch = [&](int id, int which, uint4 (&x)[PASSES]) {
             const int8_t* src = a.c.pages + (((long long)id * a.c.H + head) * 2 + which) * (kPage * HD) + row0 * HD + c * 16;
 #pragma unroll
@@ -320,8 +317,8 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
                 const uint32_t u[4] = {x[j].x ^ 0x80808080u, x[j].y ^ 0x80808080u, x[j].z ^ 0x80808080u, x[j].w ^ 0x80808080u};
                 const uint4 lo = make_uint4(halves(u[0], 0x4140), halves(u[0], 0x4342), halves(u[1], 0x4140), halves(u[1], 0x4342));
                 const uint4 hi = make_uint4(halves(u[2], 0x4140), halves(u[2], 0x4342), halves(u[3], 0x4140), halves(u[3], 0x4342));
-                *reinterpret_cast<uint4*>(dst + at0 + j * RPP * 128) = swap ? hi : lo;
-                *reinterpret_cast<uint4*>(dst + at1 + j * RPP * 128) = swap ? lo : hi;
+                *reinterpret_cast<uint4*>(dst + at0 + j * RPP * 128) = lo;
+                *reinterpret_cast<uint4*>(dst + at1 + j * RPP * 128) = hi;
             }
             fence_async_smem();
             __syncwarp();
@@ -415,70 +412,83 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
         const int all_see = __reduce_min_sync(0xffffffffu, open);
         float m = -INFINITY, l = 0.f, vr = 0.f;
         // One step: the 64 scores of a row stay in registers.
-        auto step = [&](auto masked, int i) {
-            constexpr bool MASKED = decltype(masked)::value;
+        auto step = [&](int i) {
             const float4* blk = s_blk + (i % kT8Ring) * kT8Blks;
             const float vr_now = s_vr[i % kT8Ring].x;
             const uint32_t s_at = lanes + (uint32_t)((2 * tile + (i & 1)) * kT8Keys);
             const int k0 = i * kT8Keys;
-            uint32_t sv[64];
-            tc_ld32_async(s_at, sv);
-            tc_ld32_async(s_at + 32, sv + 32);
-            tc_wait_ld64(sv);
-            if (MASKED) {
+            // In its first step a row needs a maximum to begin with; in its last one or two the keys behind it, which the block that its
+            // own key lies in holds, get -inf in S.  (Whole blocks behind it do not count, see below.)
+            const bool masked = k0 + kT8Keys - 1 > all_see;    // the same for the whole warp
+            if (i == 0 || masked) {
+                float mx = -INFINITY;
+#pragma unroll 1
+                for (int b = 0; b < kT8Blks; ++b) {
+                    uint32_t x[16];
+                    tc_ld16(s_at + b * 16, x);
+                    float top = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < 64; ++j)
-                    if (k0 + j > open) sv[j] = 0xff800000u;
+                    for (int j = 0; j < 16; ++j) {
+                        if (k0 + b * 16 + j > open) x[j] = 0xff800000u;
+                        top = fmaxf(top, __uint_as_float(x[j]));
+                    }
+                    if (masked) tc_st16(s_at + b * 16, x);
+                    mx = fmaxf(mx, fmaf(top, fmaxf(blk[b].x * row_f, 1e-37f), blk[b].w));
+                }
+                tc_wait_st();
+                if (i == 0) { m = mx; vr = vr_now; }
             }
-            // Weights against the m there is, beside their maximum: the exponentials need not wait for it.  Where a row has passed
-            // m by too much (in its first step, and rarely later), m moves and the weights are computed once more.
+            // Weights against the m there is, and beside them their maximum, which the exponentials so need not wait for.  Where a row has
+            // passed m by too much (in its first step, and rarely later), m moves and the step is done again: S is still there.
+            uint32_t pk[32];
             float l_add;
             for (;;) {
+                uint32_t sv[64];
+                tc_ld32_async(s_at, sv);
+                tc_ld32_async(s_at + 32, sv + 32);
+                tc_wait_ld64(sv);
                 const float m_use = m == -INFINITY ? 0.f : m;
                 float mx = -INFINITY;
                 l_add = 0.f;
-                uint32_t pk[16];
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     const float4 f = blk[b];
-                    const float c = f.x * row_f, d = f.y - m_use;
+                    // c stays above zero so that -inf stays -inf (a block's factor that is NaN comes by f.y); a block behind the row
+                    // does not count, whatever it holds
+                    const bool behind = k0 + b * 16 > open;
+                    const float c = fmaxf(f.x * row_f, 1e-37f), d = behind ? -INFINITY : f.y - m_use;
                     float t4[2] = {__uint_as_float(sv[b * 16]), __uint_as_float(sv[b * 16 + 1])};
 #pragma unroll
                     for (int j = 2; j < 16; j += 4) {
                         t4[0] = fmaxf(fmaxf(t4[0], __uint_as_float(sv[b * 16 + j])), __uint_as_float(sv[b * 16 + j + 1]));
                         if (j + 2 < 16) t4[1] = fmaxf(fmaxf(t4[1], __uint_as_float(sv[b * 16 + j + 2])), __uint_as_float(sv[b * 16 + j + 3]));
                     }
-                    mx = fmaxf(mx, fmaf(fmaxf(t4[0], t4[1]), c, f.w));
+                    mx = fmaxf(mx, fmaf(fmaxf(t4[0], t4[1]), c, behind ? -INFINITY : f.w));
                     const unsigned long long c2 = pair2(c, c), d2 = pair2(d, d);
                     unsigned long long sum = 0;
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
                         const float2 x = unpair2(fma2(pair2(__uint_as_float(sv[b * 16 + j]), __uint_as_float(sv[b * 16 + j + 1])), c2, d2));
-                        float w0 = exp2_fast(x.x), w1 = exp2_fast(x.y);
-                        if (MASKED) {                      // also where a factor is NaN
-                            if (k0 + b * 16 + j > open) w0 = 0.f;
-                            if (k0 + b * 16 + j + 1 > open) w1 = 0.f;
-                        }
+                        const float w0 = exp2_fast(x.x), w1 = exp2_fast(x.y);
                         sum = add2(sum, pair2(w0, w1));
-                        pk[(b & 1) * 8 + j / 2] = pack_half(w0, w1);
+                        pk[b * 8 + j / 2] = pack_half(w0, w1);
                     }
                     const float2 s2 = unpair2(sum);
                     l_add = fmaf(s2.x + s2.y, f.z, l_add);
-                    if (b & 1) tc_st16(s_at + (b >> 1) * 16, pk);       // over columns of S that this thread has read
                 }
                 const bool moves = mx > m + kT8Slack || (m == -INFINITY && mx > m);
                 if (!__any_sync(0xffffffffu, moves || vr_now != vr)) break;
                 const float m_new = moves ? mx : m;
                 const float corr = m == -INFINITY ? 0.f : exp2_fast(m - m_new);
                 l *= corr;
-                uint32_t x[16];
-                if (i > 0) {                               // O is still as the products left it: the last of them has to be done
+                if (i > 0) {                                   // O as the products so far leave it: the last of them has to be done
                     if (ok) ok = wait8(B(PV_DONE + 2 * tile + ((i - 1) & 1)), ((i - 1) >> 1) & 1);
                     ok = __all_sync(0xffffffffu, ok);
                     tc_fence_after();
                     const float f = corr * (vr_now > 0.f ? vr / vr_now : 1.f);
 #pragma unroll 1
                     for (int c = 0; c < HD / 16; ++c) {
+                        uint32_t x[16];
                         tc_ld16(o_at + c * 16, x);
 #pragma unroll
                         for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * f);
@@ -489,14 +499,15 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
                 vr = vr_now;
             }
             l += l_add;
+            tc_st16(s_at, pk);                                 // over columns of S that this thread has read
+            tc_st16(s_at + 16, pk + 16);
         };
         for (int i = 0; i < my_steps && ok; ++i) {
             ok = wait8(B(SC_FULL + i % kT8Ring), (i / kT8Ring) & 1) && wait8(B(S_READY + 2 * tile + (i & 1)), (i >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            if (i * kT8Keys + kT8Keys - 1 > all_see) step(std::integral_constant<bool, true>{}, i);     // the same for the whole warp
-            else step(std::integral_constant<bool, false>{}, i);
+            step(i);
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
