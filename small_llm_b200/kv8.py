@@ -14,36 +14,29 @@ Bad arguments raise ValueError; there is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+from struct import Struct
 
 import torch
+from torch._C import _cuda_getCurrentRawStream as _raw_stream
+from torch._C import _cuda_getDevice as _current_device
 
 from .api import _raise, load_library
 
 PAGE, BLOCK = 64, 16
 MAX_SEQS = 8192
+_I32, _I64, _I8, _F32 = torch.int32, torch.int64, torch.int8, torch.float32
 _ROWS = {torch.bfloat16: 0, torch.float32: 1}
 _HEAD_DIMS = (16, 32, 64, 128)
 
-
-class _Layer(C.Structure):
-    _fields_ = [("pages", C.c_void_p), ("scales", C.c_void_p), ("n_pages", C.c_uint64), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32)]
-
-
-class _Tables(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("len_before", "len_after", "table", "ring", "pool_in", "pool_out", "cu_tok", "tok_seq", "tok_pos", "slot_map")] + [
-        ("n_pages", C.c_uint64), ("n_seq", C.c_uint32), ("table_width", C.c_uint32), ("max_tok", C.c_uint32)]
-
-
-class _Rows(C.Structure):
-    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("slot_map", C.c_void_p), ("k_stride", C.c_uint64), ("v_stride", C.c_uint64), ("n_tok", C.c_uint32),
-                ("dtype", C.c_uint32)]
-
-
-class _Attn(C.Structure):
-    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_uint64), ("out_stride", C.c_uint64)] + [
-        (n, C.c_void_p) for n in ("table", "tok_seq", "tok_pos", "cu_tok", "status")] + [
-        (n, C.c_uint32) for n in ("n_tok", "n_seq", "table_width", "n_heads", "max_new", "max_len", "dtype")] + [("scale", C.c_float)]
-
+# The structures of include/sllm.h in their field order, packed with native alignment (packing takes a fraction of what filling
+# a ctypes structure does, which a decode step would notice).
+STRUCTS = {
+    "sllm_kv8_layer": ("@QQQII", "pages scales n_pages kv_heads head_dim"),
+    "sllm_block_tables": ("@10QQIII0Q", "len_before len_after table ring pool_in pool_out cu_tok tok_seq tok_pos slot_map n_pages n_seq table_width max_tok"),
+    "sllm_kv8_rows": ("@QQQQQII", "k v slot_map k_stride v_stride n_tok dtype"),
+    "sllm_kv8_attn": ("@QQQQQQQQQIIIIIIIf0Q", "q out q_stride out_stride table tok_seq tok_pos cu_tok status n_tok n_seq table_width n_heads max_new max_len dtype scale"),
+}
+_pack_layer, _pack_tables, _pack_rows, _pack_attn = (Struct(f).pack for f, _ in STRUCTS.values())
 
 _fns = None
 _workspaces: dict[tuple, int] = {}       # sizes of the call, device included -> bytes of workspace
@@ -67,41 +60,43 @@ def _need(ok: bool, why: str):
         raise ValueError(why)
 
 
-def _call(dev: torch.device, fn, *args):
-    """fn(*args, stream) on `dev`, which need not be the current device."""
-    i = dev.index
-    if torch.cuda.current_device() != i:
-        with torch.cuda.device(i):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+def _call(dev: int, fn, *args):
+    """fn(*args, stream) on device `dev`, which need not be the current one."""
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
     else:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+        rc = fn(*args, _raw_stream(dev))
     if rc:
         _raise(rc, _lib().sllm_last_error(None).decode())
 
 
-def _ints(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, dev: torch.device) -> int:
-    if t.dtype != dtype or t.shape != shape or t.device != dev or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {dev}")
+def _flat(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, dev: int) -> int:
+    """The address of a contiguous tensor of this type and shape on this device."""
+    if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous() or t.shape != shape:
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{dev}")
     return t.data_ptr()
 
 
-def _layer(pages: torch.Tensor, scales: torch.Tensor) -> _Layer:
-    _need(pages.is_cuda, "pages must be a CUDA tensor: this package has no CPU path")
+def _layer(pages: torch.Tensor, scales: torch.Tensor) -> tuple[bytes, int, int, int]:
+    """The packed layer, its device, heads and head_dim."""
     s = pages.shape
-    _need(pages.dtype == torch.int8 and len(s) == 5 and s[2] == 2 and s[3] == PAGE and pages.is_contiguous(),
-          "pages must be a contiguous int8 tensor [n_pages][kv_heads][2][64][head_dim]")
-    _need(s[4] in _HEAD_DIMS, "head_dim must be 16, 32, 64 or 128")
-    _need(s[0] > 0 and s[1] > 0, "a cache has at least one page and one head")
-    return _Layer(pages.data_ptr(), _ints("scales", scales, torch.float32, (s[0], s[1], 2, PAGE // BLOCK), pages.device), s[0], s[1], s[4])
+    if not (pages.is_cuda and pages.dtype is _I8 and len(s) == 5 and s[2] == 2 and s[3] == PAGE and s[4] in _HEAD_DIMS and s[0] > 0 and s[1] > 0 and pages.is_contiguous()):
+        _need(pages.is_cuda, "pages must be a CUDA tensor: this package has no CPU path")
+        _need(len(s) != 5 or s[4] in _HEAD_DIMS, "head_dim must be 16, 32, 64 or 128")
+        raise ValueError("pages must be a contiguous int8 tensor [n_pages][kv_heads][2][64][head_dim] with at least one page and one head")
+    dev, n, h, d = pages.get_device(), s[0], s[1], s[4]
+    return _pack_layer(pages.data_ptr(), _flat("scales", scales, _F32, (n, h, 2, PAGE // BLOCK), dev), n, h, d), dev, h, d
 
 
-def _rows(name: str, t: torch.Tensor, n: int, heads: int, head_dim: int, dev: torch.device) -> int:
+def _rows(name: str, t: torch.Tensor, n: int, heads: int, head_dim: int, dev: int) -> int:
     """The distance between rows, in elements."""
-    _need(t.shape == (n, heads, head_dim) and t.device == dev, f"{name} must be [{n}, {heads}, {head_dim}] on {dev}")
-    st = t.stride()
     row = heads * head_dim
-    _need(n == 0 or (st[2] == 1 and (heads == 1 or st[1] == head_dim) and (n == 1 or st[0] >= row)),
-          f"{name}: the heads of a row must be contiguous, and rows must not overlap")
+    if t.shape != (n, heads, head_dim) or t.get_device() != dev:
+        raise ValueError(f"{name} must be [{n}, {heads}, {head_dim}] on cuda:{dev}")
+    st = t.stride()
+    if n > 0 and not (st[2] == 1 and (heads == 1 or st[1] == head_dim) and (n == 1 or st[0] >= row)):
+        raise ValueError(f"{name}: the heads of a row must be contiguous, and rows must not overlap")
     return st[0] if n > 1 else row
 
 
@@ -118,45 +113,41 @@ def block_tables(len_before, len_after, table, ring, pool_in, pool_out, cu_tok, 
     table int32 [n_seq, width] and ring int32 [n_pages] are updated; pool_in int64 [4] = {head, free, -, -} is read and pool_out
     int64 [4] = {head, free, entries, status} written (another tensor); cu_tok int32 [n_seq + 1], tok_seq and tok_pos int32 [max_tok]
     and slot_map int64 [max_tok] are written whole."""
-    dev = table.device
     _need(table.is_cuda, "table must be a CUDA tensor: this package has no CPU path")
     _need(table.dim() == 2 and ring.dim() == 1 and tok_seq.dim() == 1, "table must be [n_seq, width], ring and tok_seq of one dimension")
+    dev = table.get_device()
     n, width = table.shape
-    room = tok_seq.shape
-    i32, i64 = torch.int32, torch.int64
-    a = _Tables(_ints("len_before", len_before, i32, (n,), dev), _ints("len_after", len_after, i32, (n,), dev), _ints("table", table, i32, (n, width), dev),
-                _ints("ring", ring, i32, ring.shape, dev), _ints("pool_in", pool_in, i64, (4,), dev), _ints("pool_out", pool_out, i64, (4,), dev),
-                _ints("cu_tok", cu_tok, i32, (n + 1,), dev), _ints("tok_seq", tok_seq, i32, room, dev), _ints("tok_pos", tok_pos, i32, room, dev),
-                _ints("slot_map", slot_map, i64, room, dev), ring.shape[0], n, width, room[0])
-    if room[0] == 0:                     # empty tensors have no address: any will do, nothing is written
-        a.tok_seq = a.tok_pos = a.cu_tok
-        a.slot_map = a.pool_out
-    _call(dev, _lib().sllm_k_block_tables, C.byref(a))
+    room, n_pages = tok_seq.shape[0], ring.shape[0]
+    one, entries = (n,), (room,)
+    cu, out = _flat("cu_tok", cu_tok, _I32, (n + 1,), dev), _flat("pool_out", pool_out, _I64, (4,), dev)
+    seq, pos, slot = _flat("tok_seq", tok_seq, _I32, entries, dev), _flat("tok_pos", tok_pos, _I32, entries, dev), _flat("slot_map", slot_map, _I64, entries, dev)
+    if room == 0:                        # empty tensors have no address: any will do, nothing is written
+        seq, pos, slot = cu, cu, out
+    _call(dev, _lib().sllm_k_block_tables,
+          _pack_tables(_flat("len_before", len_before, _I32, one, dev), _flat("len_after", len_after, _I32, one, dev), _flat("table", table, _I32, (n, width), dev),
+                       _flat("ring", ring, _I32, (n_pages,), dev), _flat("pool_in", pool_in, _I64, (4,), dev), out, cu, seq, pos, slot, n_pages, n, width, room))
 
 
 def append(k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor) -> None:
     """Rows k, v [n_tok, kv_heads, head_dim] (bf16 or fp32, any row stride) into the cache at slot_map int64 [n_tok]; see sllm_k_kv8_append."""
-    c = _layer(pages, scales)
-    dev, n = pages.device, k.shape[0]
-    _need(k.dtype in _ROWS and v.dtype == k.dtype, "k and v must both be bfloat16 or float32")
-    r = _Rows(k.data_ptr(), v.data_ptr(), _ints("slot_map", slot_map, torch.int64, (n,), dev), _rows("k", k, n, c.kv_heads, c.head_dim, dev),
-              _rows("v", v, n, c.kv_heads, c.head_dim, dev), n, _ROWS[k.dtype])
+    c, dev, h, d = _layer(pages, scales)
+    n, t = k.shape[0], _ROWS.get(k.dtype)
+    _need(t is not None and v.dtype is k.dtype, "k and v must both be bfloat16 or float32")
+    r = _pack_rows(k.data_ptr(), v.data_ptr(), _flat("slot_map", slot_map, _I64, (n,), dev), _rows("k", k, n, h, d, dev), _rows("v", v, n, h, d, dev), n, t)
     if n:
-        _call(dev, _lib().sllm_k_kv8_append, C.byref(c), C.byref(r))
+        _call(dev, _lib().sllm_k_kv8_append, c, r)
 
 
 def read(slots: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
     """The rows (k, v), [n, kv_heads, head_dim] each, that the cache stands for at slots int64 [n]; zeros for a slot outside the pool."""
-    c = _layer(pages, scales)
+    c, dev, h, d = _layer(pages, scales)
     _need(slots.dim() == 1, "slots must have one dimension")
-    _need(dtype in _ROWS, "dtype must be bfloat16 or float32")
-    dev, n = pages.device, slots.shape[0]
-    at = _ints("slots", slots, torch.int64, (n,), dev)
-    kv = torch.empty(2, n, c.kv_heads, c.head_dim, dtype=dtype, device=dev)
-    k, v = kv.unbind(0)
-    row = c.kv_heads * c.head_dim
+    t, n = _ROWS.get(dtype), slots.shape[0]
+    _need(t is not None, "dtype must be bfloat16 or float32")
+    at = _flat("slots", slots, _I64, (n,), dev)
+    k, v = torch.empty((2, n, h, d), dtype=dtype, device=pages.device).unbind(0)
     if n:
-        _call(dev, _lib().sllm_k_kv8_read, C.byref(c), C.byref(_Rows(k.data_ptr(), v.data_ptr(), at, row, row, n, _ROWS[dtype])))
+        _call(dev, _lib().sllm_k_kv8_read, c, _pack_rows(k.data_ptr(), v.data_ptr(), at, h * d, h * d, n, t))
     return k, v
 
 
@@ -168,35 +159,37 @@ def attention(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, table:
     Token t attends positions 0 .. tok_pos[t] of sequence tok_seq[t] (int32 [n_tok]) through table int32 [n_seq, width].  max_new and
     max_len are the most tokens a sequence has in the list and the most positions any has: they choose how the work is cut
     (0: not known).  Rows of tokens with tok_seq < 0 are left as they are, so give `out` where a list is padded."""
-    c = _layer(pages, scales)
-    dev = pages.device
+    c, dev, h, d = _layer(pages, scales)
     _need(q.dim() == 3 and table.dim() == 2, "q must be [n_tok, n_heads, head_dim], table [n_seq, width]")
     n, heads = q.shape[0], q.shape[1]
-    _need(q.dtype in _ROWS, "q must be bfloat16 or float32")
-    _need(heads > 0 and heads % c.kv_heads == 0, "n_heads must be a multiple of kv_heads")
     n_seq, width = table.shape
-    q_stride = _rows("q", q, n, heads, c.head_dim, dev)
+    t = _ROWS.get(q.dtype)
+    _need(t is not None, "q must be bfloat16 or float32")
+    _need(heads > 0 and heads % h == 0, "n_heads must be a multiple of kv_heads")
+    q_stride = _rows("q", q, n, heads, d, dev)
     if out is None:
-        out = torch.empty(n, heads, c.head_dim, dtype=q.dtype, device=dev)
-    _need(out.dtype == q.dtype, "out must have q's dtype")
+        out = torch.empty((n, heads, d), dtype=q.dtype, device=q.device)
+    _need(out.dtype is q.dtype, "out must have q's dtype")
     _need(0 <= max_new < 1 << 31 and 0 <= max_len < 1 << 31, "max_new and max_len must not be negative")
     _need(scale is None or scale != 0, "scale must not be 0")
-    i32 = torch.int32
-    a = _Attn(q.data_ptr(), out.data_ptr(), q_stride, _rows("out", out, n, heads, c.head_dim, dev), _ints("table", table, i32, (n_seq, width), dev),
-              _ints("tok_seq", tok_seq, i32, (n,), dev), _ints("tok_pos", tok_pos, i32, (n,), dev),
-              None if cu_tok is None else _ints("cu_tok", cu_tok, i32, (n_seq + 1,), dev), None if status is None else _ints("status", status, i32, (1,), dev),
-              n, n_seq, width, heads, max_new, max_len, _ROWS[q.dtype], scale or 0.0)
+    a = _pack_attn(q.data_ptr(), out.data_ptr(), q_stride, _rows("out", out, n, heads, d, dev), _flat("table", table, _I32, (n_seq, width), dev),
+                   _flat("tok_seq", tok_seq, _I32, (n,), dev), _flat("tok_pos", tok_pos, _I32, (n,), dev),
+                   0 if cu_tok is None else _flat("cu_tok", cu_tok, _I32, (n_seq + 1,), dev), 0 if status is None else _flat("status", status, _I32, (1,), dev),
+                   n, n_seq, width, heads, max_new, max_len, t, scale or 0.0)
     if n == 0:
         return out
     lib = _lib()
-    key = (dev.index, c.kv_heads, c.head_dim, n, n_seq, width, heads, max_new, max_len, q.dtype, cu_tok is None)
+    key = (dev, h, d, n, n_seq, width, heads, max_new, max_len, t, cu_tok is None)
     need = _workspaces.get(key)
     if need is None:
         got = C.c_uint64()
-        _call(dev, lambda *x: lib.sllm_k_attn_kv8_workspace(*x[:-1]), C.byref(c), C.byref(a), C.byref(got))
+        _call(dev, lambda *x: lib.sllm_k_attn_kv8_workspace(*x[:-1]), c, a, C.byref(got))
         if len(_workspaces) > 4096:
             _workspaces.clear()
         need = _workspaces[key] = got.value
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(dev, lib.sllm_k_attn_kv8, C.byref(c), C.byref(a), ws.data_ptr() if need else None, need)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        _call(dev, lib.sllm_k_attn_kv8, c, a, ws.data_ptr(), need)
+    else:
+        _call(dev, lib.sllm_k_attn_kv8, c, a, None, 0)
     return out

@@ -639,13 +639,13 @@ def test_refusals():
     # the C entry itself: host memory and missing workspaces
     import ctypes as C
     lib, host = kv8._lib(), torch.zeros(4, 2, 64)
-    c = kv8._layer(pages, scales)
-    r = kv8._Rows(host.data_ptr(), k.data_ptr(), slots.data_ptr(), 128, 128, 4, 1)
-    assert lib.sllm_k_kv8_append(C.byref(c), C.byref(r), None) == 1 and b"current device" in lib.sllm_last_error(None)
+    c = kv8._layer(pages, scales)[0]
+    r = kv8._pack_rows(host.data_ptr(), k.data_ptr(), slots.data_ptr(), 128, 128, 4, 1)
+    assert lib.sllm_k_kv8_append(c, r, None) == 1 and b"current device" in lib.sllm_last_error(None)
     long = torch.zeros(1, 4000, **i32)
-    a = kv8._Attn(k.data_ptr(), torch.empty_like(k).data_ptr(), 128, 128, long.data_ptr(), seq.data_ptr(), seq.data_ptr(), None, None, 4, 1, 4000, 2, 1, 0, 1, 0.0)
+    a = kv8._pack_attn(k.data_ptr(), torch.empty_like(k).data_ptr(), 128, 128, long.data_ptr(), seq.data_ptr(), seq.data_ptr(), 0, 0, 4, 1, 4000, 2, 1, 0, 1, 0.0)
     need = C.c_uint64()
-    assert lib.sllm_k_attn_kv8_workspace(C.byref(c), C.byref(a), C.byref(need)) == 0 and need.value > 0
-    assert lib.sllm_k_attn_kv8(C.byref(c), C.byref(a), None, 0, None) == 1 and b"workspace" in lib.sllm_last_error(None)
+    assert lib.sllm_k_attn_kv8_workspace(c, a, C.byref(need)) == 0 and need.value > 0
+    assert lib.sllm_k_attn_kv8(c, a, None, 0, None) == 1 and b"workspace" in lib.sllm_last_error(None)
     ws = torch.empty(need.value, dtype=torch.uint8, device="cuda")
-    assert lib.sllm_k_attn_kv8(C.byref(c), C.byref(a), ws.data_ptr(), need.value - 1, None) == 1
+    assert lib.sllm_k_attn_kv8(c, a, ws.data_ptr(), need.value - 1, None) == 1

@@ -2,7 +2,9 @@
 any device work."""
 import ctypes as C
 import os
+import re
 import subprocess
+from struct import Struct
 
 import pytest
 import torch
@@ -11,43 +13,41 @@ import small_llm_b200 as sl
 from small_llm_b200 import kv8
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-STRUCTS = {"sllm_kv8_layer": kv8._Layer, "sllm_block_tables": kv8._Tables, "sllm_kv8_rows": kv8._Rows, "sllm_kv8_attn": kv8._Attn}
-
-
 def test_structures_match_the_header(tmp_path):
     lines = []
-    for name, s in STRUCTS.items():
+    for name, (_, fields) in kv8.STRUCTS.items():
         lines.append(f'printf("{name} %zu\\n", sizeof({name}));')
-        lines += [f'printf("{name}.{f} %zu\\n", offsetof({name}, {f}));' for f, _ in s._fields_]
+        lines += [f'printf("{name}.{f} %zu %zu\\n", offsetof({name}, {f}), sizeof((({name}*)0)->{f}));' for f in fields.split()]
     src = tmp_path / "s.c"
-    src.write_text('#include <stdio.h>\n#include "sllm.h"\nint main(void) {' + "\n".join(lines) + "return 0;}\n")
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "sllm.h"\nint main(void) {' + "\n".join(lines) + "return 0;}\n")
     subprocess.run(["gcc", "-std=c11", "-Wall", "-Werror", f"-I{ROOT}/include", str(src), "-o", str(tmp_path / "s")], check=True)
-    got = dict(line.split() for line in subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.splitlines())
-    for name, s in STRUCTS.items():
-        assert int(got[name]) == C.sizeof(s)
-        for f, _ in s._fields_:
-            assert int(got[f"{name}.{f}"]) == getattr(s, f).offset
+    got = {k: v for k, *v in (line.split() for line in subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.splitlines())}
+    for name, (fmt, fields) in kv8.STRUCTS.items():
+        assert int(got[name][0]) == Struct(fmt).size
+        at = 0
+        for f, letter in zip(fields.split(), "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([A-Za-z])", fmt) if n != "0")):
+            size = Struct(letter).size
+            at = -(-at // size) * size
+            assert [int(x) for x in got[f"{name}.{f}"]] == [at, size], (name, f)
+            at += size
+
+
+def _packed(name, values, over):
+    fmt, fields = kv8.STRUCTS[name]
+    v = dict(zip(fields.split(), values)) | {k: x or 0 for k, x in over.items()}
+    return Struct(fmt).pack(*v.values())
 
 
 def _layer(**over):
-    c = kv8._Layer(1 << 20, 2 << 20, 4, 2, 64)
-    for k, v in over.items():
-        setattr(c, k, v)
-    return c
+    return _packed("sllm_kv8_layer", (1 << 20, 2 << 20, 4, 2, 64), over)
 
 
 def _attn(**over):
-    a = kv8._Attn(1 << 24, 1 << 26, 256, 256, 4096, 8192, 8192, None, None, 3, 2, 8, 4, 1, 100, 0, 0.0)
-    for k, v in over.items():
-        setattr(a, k, v)
-    return a
+    return _packed("sllm_kv8_attn", (1 << 24, 1 << 26, 256, 256, 4096, 8192, 8192, 0, 0, 3, 2, 8, 4, 1, 100, 0, 0.0), over)
 
 
 def _rows(**over):
-    r = kv8._Rows(1 << 24, 1 << 26, 4096, 128, 128, 3, 0)
-    for k, v in over.items():
-        setattr(r, k, v)
-    return r
+    return _packed("sllm_kv8_rows", (1 << 24, 1 << 26, 4096, 128, 128, 3, 0), over)
 
 
 def _refused(fn, *args):
@@ -62,10 +62,10 @@ def _refused(fn, *args):
 def test_layers_refused(over, why):
     lib = kv8._lib()
     c, got = _layer(**over), C.c_uint64()
-    assert why in _refused(lib.sllm_k_kv8_append, C.byref(c), C.byref(_rows()), None)
-    assert why in _refused(lib.sllm_k_kv8_read, C.byref(c), C.byref(_rows()), None)
-    assert why in _refused(lib.sllm_k_attn_kv8, C.byref(c), C.byref(_attn()), None, 0, None)
-    assert why in _refused(lib.sllm_k_attn_kv8_workspace, C.byref(c), C.byref(_attn()), C.byref(got))
+    assert why in _refused(lib.sllm_k_kv8_append, c, _rows(), None)
+    assert why in _refused(lib.sllm_k_kv8_read, c, _rows(), None)
+    assert why in _refused(lib.sllm_k_attn_kv8, c, _attn(), None, 0, None)
+    assert why in _refused(lib.sllm_k_attn_kv8_workspace, c, _attn(), C.byref(got))
 
 
 @pytest.mark.parametrize("over,why", [
@@ -73,8 +73,8 @@ def test_layers_refused(over, why):
     (dict(n_tok=0x40000001), "too many"), (dict(k=(1 << 24) + 1), "misaligned"), (dict(slot_map=4100), "misaligned")])
 def test_rows_refused(over, why):
     lib = kv8._lib()
-    assert why in _refused(lib.sllm_k_kv8_append, C.byref(_layer()), C.byref(_rows(**over)), None)
-    assert why in _refused(lib.sllm_k_kv8_read, C.byref(_layer()), C.byref(_rows(**over)), None)
+    assert why in _refused(lib.sllm_k_kv8_append, _layer(), _rows(**over), None)
+    assert why in _refused(lib.sllm_k_kv8_read, _layer(), _rows(**over), None)
 
 
 @pytest.mark.parametrize("over,why", [
@@ -84,17 +84,15 @@ def test_rows_refused(over, why):
     (dict(out=(1 << 24) + 512), "overlap"), (dict(tok_pos=8194), "misaligned")])
 def test_queries_refused(over, why):
     lib = kv8._lib()
-    assert why in _refused(lib.sllm_k_attn_kv8, C.byref(_layer()), C.byref(_attn(**over)), None, 0, None)
+    assert why in _refused(lib.sllm_k_attn_kv8, _layer(), _attn(**over), None, 0, None)
 
 
 @pytest.mark.parametrize("over,why", [
     (dict(len_before=None), "null"), (dict(slot_map=None), "null"), (dict(n_seq=0), "n_seq"), (dict(n_seq=8193), "n_seq"), (dict(table_width=0), "table_width"),
     (dict(n_pages=0), "n_pages"), (dict(pool_out=4096), "overlap"), (dict(pool_out=4096 + 24), "overlap"), (dict(ring=4098), "misaligned")])
 def test_tables_refused(over, why):
-    a = kv8._Tables(*[4096] * 5, 8192, *[4096] * 4, 10, 2, 4, 16)
-    for k, v in over.items():
-        setattr(a, k, v)
-    assert why in _refused(kv8._lib().sllm_k_block_tables, C.byref(a), None)
+    a = _packed("sllm_block_tables", (*[4096] * 5, 8192, *[4096] * 4, 10, 2, 4, 16), over)
+    assert why in _refused(kv8._lib().sllm_k_block_tables, a, None)
 
 
 def test_no_cpu_path():
@@ -106,4 +104,4 @@ def test_no_cpu_path():
     with pytest.raises(ValueError, match="head_dim"):
         kv8.empty_cache(1, 1, 80, device="cpu")
     if not torch.cuda.is_available():
-        assert kv8._lib().sllm_k_attn_kv8(C.byref(_layer()), C.byref(_attn()), None, 0, None) == 3      # SLLM_ERR_CUDA: no device
+        assert kv8._lib().sllm_k_attn_kv8(_layer(), _attn(), None, 0, None) == 3      # SLLM_ERR_CUDA: no device
