@@ -4,20 +4,26 @@
 //   o = sum_j p_j vs_b(j) V_j / sum_j p_j,   p_j = exp(scale ks_b(j) (q . K_j) - m),   j <= position of the row
 //
 // with K_j, V_j the stored integers and ks, vs the scales of their blocks of 16 positions.  Only a block's scale touches an
-// integer product, so the products run on the integers themselves, which are exact in fp16: mma.sync m16n8k16 with eight
-// query rows (tokens x heads that share a kv head) as its rows 0..7, and fp32 accumulators.  Rows 8..15 carry what fp16
-// rounds away: q and p are split into a high and a low fp16 part (22 bits), both products come out in the same thread
-// and are added there.  q is first divided by a power of two so that its largest value is in [0.5, 1); p vs is divided by
-// vr, a power of two no smaller than the largest vs so far, which is carried like the running maximum m.  So fp32 queries
-// keep fp32 accuracy, at no more matrix instructions than one row costs.
+// integer product, so the products run on the integers themselves: mma.sync with eight query rows (tokens x heads that share
+// a kv head) as its rows 0..7, and what the 8 or 11 bits of an operand leave out of them as its rows 8..15, so that both parts
+// come out in one thread and are added there, at no more matrix instructions than one row costs.  q is first divided by a power
+// of two so that its largest value is in [0.5, 1); p vs is divided by vr, a power of two no smaller than the largest vs so far,
+// which is carried like the running maximum m.  Two forms:
+//   bf16 rows (I8): m16n8k32 on int8, the cache's bytes as they are.  q and p vs / vr become two base-256 digits, 16 bits in
+//     all (2^-16 of the row's largest value: bf16 has 2^-9 of each; 2^-16 of a weight of 1, each key's own, against an output rounded
+//     to 2^-9); products are exact, sums are 32-bit integers.
+//   fp32 rows: m16n8k16 on fp16, in which the integers are exact, q and p vs / vr split into a high and a low fp16 part, 22
+//     bits, fp32 sums: fp32 accuracy.  A byte costs 1.25-1.5 instructions on its way there (xor the sign, byte-permute under 0x64
+//     = 1024 + x, subtract), where I8 spends none on K and half of one on V, to bring four keys of a dim into one register.
 //
-// The kernel is bound by HBM: 2 head_dim bytes per cached position and kv head.  An int8 in the cache costs about 1.4
-// instructions on its way to the matrix unit (xor the sign, byte-permute under 0x64 = 1024 + x, subtract), a fraction of what a scalar
-// dot product would.  A block of threads takes one (row tile, kv head, chunk of the keys); each of its four warps takes every
-// fourth unit of 32 keys, through bulk copies of its own, three units ahead, and has its own running state; the states
-// are joined once.  Keys are cut into chunks when there are few rows; a second, small kernel joins the chunks.
+// The kernel is to be bound by HBM: 2 head_dim bytes per cached position and kv head.  A block of threads takes one (row
+// tile, kv head, chunk of the keys); each of its four warps takes every fourth unit of 32 keys, through bulk copies of its own,
+// three units ahead, and has its own running state; the states are joined once.  Keys are cut into chunks when there are few
+// rows; a second, small kernel joins the chunks.
 #pragma once
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "attn_stream.cuh"
 #include "kv8.cuh"
@@ -58,6 +64,20 @@ template <int HD> __host__ __device__ constexpr size_t attn8_smem() {
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16832(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Four values in [-1, 1] times 32512, rounded, as two base-256 digits each: the high ones in [-127, 127], the low ones in
+// [-128, 127].  The sum with 1.5 * 2^23 + 128 leaves the integer, 128 up, in the low bits: its second byte is the high digit and
+// its first, sign flipped, the low one.
+constexpr float kDigits = 32512.f;
+__device__ __forceinline__ uint32_t digit_bits(float x, float f) { return __float_as_uint(fmaf(x, f, 12583040.f)); }
+__device__ __forceinline__ void digits4(uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3, uint32_t& hi, uint32_t& lo) {
+    const uint32_t a = __byte_perm(x0, x1, 0x5140), b = __byte_perm(x2, x3, 0x5140);      // low, low, high, high
+    lo = __byte_perm(a, b, 0x5410) ^ 0x80808080u;
+    hi = __byte_perm(a, b, 0x7632);
 }
 // bytes 0, 1 (or 2, 3) of four excess-128 bytes as two halves: 0x64xx is 1024 + xx, minus 1152 leaves the signed value
 __device__ __forceinline__ uint32_t halves(uint32_t w, uint32_t sel) {
@@ -109,9 +129,10 @@ __device__ __forceinline__ int attn8_tile(const Attn8Args& a, int tile, int& t0,
 // chunks of a tile whose last row stands at `last`
 __device__ __forceinline__ int attn8_chunks(const Attn8Args& a, int last) { return min((last + a.chunk) / a.chunk, a.n_chunks); }
 
-template <typename T, int HD>
+template <typename T, int HD, bool I8>
 __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
-    constexpr int KS = HD / 16;                  // k steps of the score product
+    static_assert(!I8 || HD >= 32, "a k step of the integer products has 32 dims");
+    constexpr int KS = HD / (I8 ? 32 : 16);      // k steps of the score product
     constexpr int KB = HD / 4;                   // bytes of a key row per lane
     constexpr int VB = HD / 8;                   // bytes of a value row per lane = column tiles of the output
     constexpr uint32_t RUN = kA8Unit * HD;       // bytes of a unit's K (or V) rows
@@ -170,6 +191,23 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
         const int e = min(max((int)(__float_as_uint(top) >> 23) - 126, -125), 125);
         const float f = top > 0.f ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
         row_f = (top > 0.f ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f) * a.scale * 1.4426950408889634f;
+        if constexpr (I8) {
+            // digits know no infinity and no NaN: the row's factor carries them
+            float odd = 0.f;
+#pragma unroll
+            for (int i = 0; i < KB; ++i) odd = fmaf(x[i], 0.f, odd);
+            odd += __shfl_xor_sync(0xffffffffu, odd, 1);
+            odd += __shfl_xor_sync(0xffffffffu, odd, 2);
+            row_f = row_f * (1.f / kDigits) + odd;
+            const float fd = row_ok ? f * kDigits : 0.f;
+#pragma unroll
+            for (int j = 0; j < KS; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float* y = x + 8 * j + 4 * h;
+                    digits4(digit_bits(y[0], fd), digit_bits(y[1], fd), digit_bits(y[2], fd), digit_bits(y[3], fd), qa[j][2 * h], qa[j][2 * h + 1]);
+                }
+        } else
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
             if (!row_ok) { x[4 * j] = x[4 * j + 1] = x[4 * j + 2] = x[4 * j + 3] = 0.f; }
@@ -178,9 +216,10 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
         }
     }
 
-    float o[VB][4];
+    using Acc = typename std::conditional<I8, int, float>::type;
+    Acc o[VB][4];
 #pragma unroll
-    for (int j = 0; j < VB; ++j) { o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f; }
+    for (int j = 0; j < VB; ++j) { o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0; }
     float m_run = -INFINITY, l_run = 0.f, vr = 0.f, vr_inv = 0.f;
 
     const int n_units = keys > 0 ? (keys + kA8Unit - 1) / kA8Unit : 0;
@@ -231,10 +270,10 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
             const int unit = i * kA8Warps + warp;
             const float* scl = reinterpret_cast<const float*>(sk + 2 * RUN) + (unit % (kPage / kA8Unit)) * 2;
             const int kb = k0 + unit * kA8Unit;                  // first key of the unit
-            float sc[4][4];
+            float sc[4][2];
 #pragma unroll
             for (int nt = 0; nt < 4; ++nt) {
-                sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+                Acc part[4] = {0, 0, 0, 0};
                 uint32_t w[KB / 4];
                 const unsigned char* row = sk + (nt * 8 + key_of_g) * HD + t * KB;
                 if constexpr (KB >= 16) {
@@ -244,9 +283,14 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
                 else w[0] = *reinterpret_cast<const uint32_t*>(row);
 #pragma unroll
                 for (int j = 0; j < KS; ++j) {
-                    const uint32_t b = w[j] ^ 0x80808080u;
-                    mma16816(sc[nt], qa[j], halves(b, 0x4140), halves(b, 0x4342));
+                    if constexpr (I8) mma16832(part, qa[j], w[2 * j], w[2 * j + 1]);
+                    else {
+                        const uint32_t b = w[j] ^ 0x80808080u;
+                        mma16816(part, qa[j], halves(b, 0x4140), halves(b, 0x4342));
+                    }
                 }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) sc[nt][e] = I8 ? (float)((int)part[e] * 256 + (int)part[e + 2]) : (float)part[e] + (float)part[e + 2];
             }
             // scores in units of log2(e), masked by selection: what stands in a masked place is never used
             float mx = -INFINITY;
@@ -256,20 +300,22 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int key = kb + nt * 8 + ((2 * t + e) ^ (t >> 1));
-                    sc[nt][e] = key <= pos ? (sc[nt][e] + sc[nt][e + 2]) * f : -INFINITY;
+                    sc[nt][e] = key <= pos ? sc[nt][e] * f : -INFINITY;
                     mx = fmaxf(mx, sc[nt][e]);
                 }
             }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float m_new = fmaxf(m_run, mx);
+            // The integer form's weights must not pass 1: m moves a little further than it has to, and so less often.
+            const float m_new = mx > m_run ? (I8 ? mx + 1.f : mx) : m_run;
             const float m_use = m_new == -INFINITY ? 0.f : m_new;
             float corr = exp2_fast(m_run - m_use);
+            if (I8 && m_run == m_new) corr = 1.f;                // also where both are -inf
             m_run = m_new;
             l_run *= corr;
-            const float vs0 = scl[4], vs1 = scl[5];
             // the second block of a unit may lie behind the last position: its scale is another owner's then and does not count
-            const float vtop = kb + kBlk8 <= last ? fmaxf(vs0, vs1) : vs0;
+            const float vs0 = scl[4], vs1 = kb + kBlk8 <= last ? scl[5] : 0.f;
+            const float vtop = fmaxf(vs0, vs1);
             if (vtop > vr) {
                 const float up = pow2_above(fminf(vtop, 1.7e38f));
                 corr *= vr / up;
@@ -278,8 +324,55 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
             }
             if (__any_sync(0xffffffffu, corr != 1.f)) {
 #pragma unroll
-                for (int j = 0; j < VB; ++j) { o[j][0] *= corr; o[j][1] *= corr; o[j][2] *= corr; o[j][3] *= corr; }
+                for (int j = 0; j < VB; ++j)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if constexpr (I8) o[j][k] = __float2int_rn((float)o[j][k] * corr);       // half a unit off: 2^-16 of one key's weight
+                        else o[j][k] *= corr;
             }
+            if constexpr (I8) {
+                // digits carry no NaN: a scale that is one shows by way of the sum
+                if (vs0 != vs0 && kb <= pos) l_run = vs0;
+                if (vs1 != vs1 && kb + kBlk8 <= pos) l_run = vs1;
+                uint32_t pa[4], x[8];
+#pragma unroll
+                for (int nt = 0; nt < 4; ++nt) {
+                    const float vf = (nt >> 1 ? vs1 : vs0) * vr_inv * kDigits;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float p = exp2_fast(sc[nt][e] - m_use);
+                        l_run += p;
+                        x[2 * nt + e] = digit_bits(p, vf);
+                    }
+                }
+                digits4(x[0], x[1], x[2], x[3], pa[0], pa[1]);
+                digits4(x[4], x[5], x[6], x[7], pa[2], pa[3]);
+                // V: eight keys' rows, (2t, 2t + 1) of each group of 8 as permuted above; four bytes of four rows are turned into four
+                // keys of four dims
+                constexpr int NW = VB / 4;
+                const int e0 = (2 * t) ^ (t >> 1), e1 = (2 * t + 1) ^ (t >> 1);
+                uint32_t v[8][NW];
+#pragma unroll
+                for (int y = 0; y < 8; ++y) {
+                    const unsigned char* src = sv + ((y & 1 ? e1 : e0) + (y >> 1) * 8) * HD + g * VB;
+                    if constexpr (NW == 4) *reinterpret_cast<uint4*>(v[y]) = *reinterpret_cast<const uint4*>(src);
+                    else if constexpr (NW == 2) *reinterpret_cast<uint2*>(v[y]) = *reinterpret_cast<const uint2*>(src);
+                    else v[y][0] = *reinterpret_cast<const uint32_t*>(src);
+                }
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    uint32_t b[2][4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t r0 = __byte_perm(v[4 * h][w], v[4 * h + 1][w], 0x5140), r1 = __byte_perm(v[4 * h][w], v[4 * h + 1][w], 0x7362);
+                        const uint32_t r2 = __byte_perm(v[4 * h + 2][w], v[4 * h + 3][w], 0x5140), r3 = __byte_perm(v[4 * h + 2][w], v[4 * h + 3][w], 0x7362);
+                        b[h][0] = __byte_perm(r0, r2, 0x5410); b[h][1] = __byte_perm(r0, r2, 0x7632);
+                        b[h][2] = __byte_perm(r1, r3, 0x5410); b[h][3] = __byte_perm(r1, r3, 0x7632);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma16832(o[4 * w + k], pa, b[0][k], b[1][k]);
+                }
+            } else {
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
                 const float vf = (kk ? vs1 : vs0) * vr_inv;
@@ -327,6 +420,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
                     mma16816(o[1], pa, halves(a0, 0x4342), halves(b0, 0x4342));
                 }
             }
+            }
             __syncwarp();                                        // every lane is done with stage s
         }
         if (i + kA8Stages < mine) issue(i + kA8Stages);
@@ -347,7 +441,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     for (int j = 0; j < VB; ++j)
 #pragma unroll
         for (int e = 0; e < 2; ++e)                              // column 2t + e of column tile j is dim (2t + e) VB + j
-            so[(warp * kA8Rows + g) * OS + (2 * t + e) * VB + j] = (o[j][e] + o[j][e + 2]) * vr;
+            so[(warp * kA8Rows + g) * OS + (2 * t + e) * VB + j] = I8 ? fmaf((float)o[j][e], 256.f, (float)o[j][e + 2]) * (vr * (1.f / kDigits)) : (o[j][e] + o[j][e + 2]) * vr;
     __syncthreads();
     // eight dims per thread at a time: the four states joined in the order of the warps
     for (int x = tid; x < kA8Rows * HD / 8; x += kA8Threads) {

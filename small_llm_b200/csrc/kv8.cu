@@ -194,16 +194,23 @@ int check_attn(const char* what, const sllm_kv8_layer* c, const sllm_kv8_attn* a
     return SLLM_OK;
 }
 
-template <typename T, int HD>
-int attn_hd(const Plan& p, int dev, void* stream) {
+template <typename T, int HD, bool I8>
+int attn_form(const Plan& p, int dev, void* stream) {
     static std::atomic<uint64_t> done{0};
     const char* what = "sllm_k_attn_kv8";
-    if (int rc = opt_in(what, k_attn_kv8<T, HD>, attn8_smem<HD>(), dev, done)) return rc;
+    if (int rc = opt_in(what, k_attn_kv8<T, HD, I8>, attn8_smem<HD>(), dev, done)) return rc;
     const Attn8Args& a = p.a;
-    if (int rc = launch(what, k_attn_kv8<T, HD>, dim3(p.tiles, a.c.H * a.head_tiles, a.n_chunks), kA8Threads, attn8_smem<HD>(), stream, a)) return rc;
+    if (int rc = launch(what, k_attn_kv8<T, HD, I8>, dim3(p.tiles, a.c.H * a.head_tiles, a.n_chunks), kA8Threads, attn8_smem<HD>(), stream, a)) return rc;
     if (a.n_chunks == 1) return SLLM_OK;
     const long long pairs = (long long)a.n_tok * a.n_heads;
     return launch(what, k_attn_kv8_join<T, HD>, dim3((unsigned)((pairs + 3) / 4)), 128, 0, stream, a);
+}
+template <typename T, int HD>
+int attn_hd(const Plan& p, int dev, void* stream) {
+    // The integer form: bf16 rows, and no more keys per warp than its 32-bit sums hold whatever they are (2^17 products of 127 * 127).
+    if constexpr (std::is_same<T, __nv_bfloat16>::value && HD >= 32)
+        if ((long long)p.a.width * kPage <= (long long)kA8Warps << 17) return attn_form<T, HD, true>(p, dev, stream);
+    return attn_form<T, HD, false>(p, dev, stream);
 }
 template <int HD, int NT>
 int attn_tc(const Plan& p, int dev, void* stream) {
