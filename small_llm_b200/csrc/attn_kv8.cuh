@@ -32,7 +32,7 @@ namespace sllm {
 
 constexpr int kA8Warps = 4;
 constexpr int kA8Threads = kA8Warps * 32;
-constexpr int kA8Stages = 3;
+constexpr int kA8Stages = 2;           // units in flight per warp: more would cost a block per SM (512 sequences: 3 stages 139 us, 2 stages 128 us)
 constexpr int kA8Unit = 32;            // keys per step of a warp: two blocks of 16
 constexpr int kA8Rows = 8;             // query rows of a tile
 
@@ -51,7 +51,8 @@ struct Attn8Args {
     int n_chunks;
     int wide;                          // q and out rows are 16-byte aligned
     float scale;
-    float* part;                       // n_chunks > 1: [n_tok][n_heads][n_chunks][hd] sums, then [..][2] (m in log2 units, l)
+    int cluster;                       // they are a cluster's blocks
+    float* part;                       // n_chunks > 1 without a cluster: [n_tok][n_heads][n_chunks][hd] sums, then [..][2] (m in log2 units, l)
     float* part_ml;
     int* status;                       // optional
 };
@@ -126,10 +127,32 @@ __device__ __forceinline__ int attn8_tile(const Attn8Args& a, int tile, int& t0,
     return first >= 0 && t0 >= 0 ? min(a.rows_toks, end - t0) : 0;
 }
 
+constexpr int kA8MaxCluster = 8;       // blocks of a cluster: what every GPU grants
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the float at the same place of shared memory in the cluster's block `rank`
+__device__ __forceinline__ float peer_f32(const float* p, int rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(as_smem(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 peer_f32x4(const float* p, int rank) {
+    uint32_t at;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(as_smem(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+// weight of a part with maximum mp and sum lp in a whole with maximum m: a part whose scores are all NaN has no maximum, but its sum says so
+__device__ __forceinline__ float part_weight(float mp, float lp, float m) { return mp == -INFINITY ? (lp == 0.f ? 0.f : 1.f) : exp2_fast(mp - m); }
 // chunks of a tile whose last row stands at `last`
 __device__ __forceinline__ int attn8_chunks(const Attn8Args& a, int last) { return min((last + a.chunk) / a.chunk, a.n_chunks); }
 
-template <typename T, int HD, bool I8>
+// CL: the chunks of a tile are a cluster's blocks (a form of its own: it costs registers, and with them blocks per SM)
+template <typename T, int HD, bool I8, bool CL>
 __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     static_assert(!I8 || HD >= 32, "a k step of the integer products has 32 dims");
     constexpr int KS = HD / (I8 ? 32 : 16);      // k steps of the score product
@@ -137,24 +160,29 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     constexpr int VB = HD / 8;                   // bytes of a value row per lane = column tiles of the output
     constexpr uint32_t RUN = kA8Unit * HD;       // bytes of a unit's K (or V) rows
     constexpr uint32_t STAGE = 2 * RUN + 64;
+    constexpr int ST = kA8Stages;
     extern __shared__ __align__(128) unsigned char smem_raw[];
-    __shared__ __align__(8) unsigned long long bars[kA8Warps][kA8Stages];
+    __shared__ __align__(8) unsigned long long bars[kA8Warps][ST];
     __shared__ float s_m[kA8Warps][kA8Rows], s_l[kA8Warps][kA8Rows];
+    __shared__ float s_cm[CL ? kA8Rows : 1], s_cl[CL ? kA8Rows : 1];
+    __shared__ __align__(16) float s_co[CL ? kA8Rows : 1][CL ? HD : 4];      // the block's joined state, for the cluster
     __shared__ int s_ok;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     if (tid == 0) {
         for (int w = 0; w < kA8Warps; ++w)
-            for (int s = 0; s < kA8Stages; ++s) bar_init(as_smem(&bars[w][s]), 1);
+            for (int s = 0; s < ST; ++s) bar_init(as_smem(&bars[w][s]), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         s_ok = 1;
     }
     pdl_launch_dependents();
     pdl_wait();
+    // heads follow on one another: the blocks that run side by side read the same pages, whose heads lie next to each other
+    const int per_tile = a.c.H * a.head_tiles, tile = blockIdx.x / per_tile, in_tile = blockIdx.x % per_tile;
     int t0, seq;
-    const int n = attn8_tile(a, blockIdx.x, t0, seq);
+    const int n = attn8_tile(a, tile, t0, seq);
     if (n <= 0) return;
-    const int head = blockIdx.y / a.head_tiles, ht = blockIdx.y % a.head_tiles;
+    const int head = in_tile / a.head_tiles, ht = in_tile % a.head_tiles;
     const int chunk = blockIdx.z;
     // this lane's row
     const int r_tok = g / a.rows_heads, r_head = ht * a.rows_heads + g % a.rows_heads;
@@ -166,7 +194,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     for (int o = 4; o < 32; o <<= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
     const int k0 = chunk * a.chunk;              // n_chunks * chunk may pass what this tile has; the last chunk takes all that is left
     const int keys = chunk == a.n_chunks - 1 ? last + 1 - k0 : min(last + 1 - k0, a.chunk);
-    if (keys <= 0 && chunk > 0) return;          // chunk 0 writes the rows that attend nothing
+    if (keys <= 0 && chunk > 0 && !CL) return;          // chunk 0 writes the rows that attend nothing
     __syncthreads();                             // barriers are initialised
 
     // the query rows as the A operand: reg 0, 2: this row's high parts; 1, 3: its low parts
@@ -225,7 +253,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     const int n_units = keys > 0 ? (keys + kA8Unit - 1) / kA8Unit : 0;
     const int mine = n_units > warp ? (n_units - warp + kA8Warps - 1) / kA8Warps : 0;
     const int* table = a.table + (size_t)seq * a.width + k0 / kPage;
-    unsigned char* my = smem_raw + (size_t)warp * kA8Stages * STAGE;
+    unsigned char* my = smem_raw + (size_t)warp * ST * STAGE;
     // pages of 32 of this warp's units at a time, one per lane; -1 stands for a page outside the pool, whose keys do not count
     auto pages_of = [&](int i0) {
         const int u = (i0 + lane) * kA8Warps + warp;
@@ -241,7 +269,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
         if ((i & 31) == 0 && i) pid_iss = pages_of(i);
         const int page = __shfl_sync(0xffffffffu, pid_iss, i & 31);
         if (page < 0 || lane != 0) return;
-        const int s = i % kA8Stages, half_page = (i * kA8Warps + warp) % (kPage / kA8Unit);
+        const int s = i % ST, half_page = (i * kA8Warps + warp) % (kPage / kA8Unit);
         const uint32_t bar = as_smem(&bars[warp][s]), dst = as_smem(my + (size_t)s * STAGE);
         const long long run = ((long long)page * a.c.H + head) * 2;
         bar_expect(bar, 2 * RUN + 32);
@@ -249,7 +277,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
         bulk_g2s(dst + RUN, a.c.pages + ((run + 1) * kPage + half_page * kA8Unit) * HD, RUN, bar);
         bulk_g2s(dst + 2 * RUN, a.c.scales + run * kBlksPerPage, 32, bar);
     };
-    for (int i = 0; i < kA8Stages && i < mine; ++i) issue(i);
+    for (int i = 0; i < ST && i < mine; ++i) issue(i);
 
     bool ok = true;
     uint32_t phase = 0;
@@ -259,7 +287,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     for (int i = 0; i < mine; ++i) {
         if ((i & 31) == 0 && i) pid_use = pages_of(i);
         const int page = __shfl_sync(0xffffffffu, pid_use, i & 31);
-        const int s = i % kA8Stages;
+        const int s = i % ST;
         if (page >= 0) {
             ok = bar_wait(as_smem(&bars[warp][s]), (phase >> s) & 1);
             ok = __all_sync(0xffffffffu, ok);
@@ -423,7 +451,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
             }
             __syncwarp();                                        // every lane is done with stage s
         }
-        if (i + kA8Stages < mine) issue(i + kA8Stages);
+        if (i + ST < mine) issue(i + ST);
     }
     if (!ok) { s_ok = 0; if (a.status) atomicExch(a.status, 5); }
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
@@ -432,7 +460,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     __syncthreads();                                             // every warp is done with its stages: their memory is used again
     if (!s_ok) {                                                 // let copies in flight land before shared memory is released
         for (int i = 0; i < 32; ++i) __nanosleep(16384);
-        return;
+        if (!CL) return;                                  // the cluster's other blocks are at its barriers
     }
     constexpr int OS = HD + 4;                                   // floats per row: rows start in different banks
     static_assert((size_t)kA8Warps * kA8Rows * OS * 4 <= attn8_smem<HD>(), "the joined states fit the stages");
@@ -454,8 +482,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
         float l = 0.f, f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < kA8Warps; ++w) {
-            // a state whose scores are all NaN has no maximum, but its sum says so
-            const float wt = s_m[w][r] == -INFINITY ? (s_l[w][r] == 0.f ? 0.f : 1.f) : exp2_fast(s_m[w][r] - m);
+            const float wt = part_weight(s_m[w][r], s_l[w][r], m);
             if (wt == 0.f && s_l[w][r] == 0.f) continue;
             l += wt * s_l[w][r];
 #pragma unroll
@@ -463,8 +490,10 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
         }
         const long long tok = t0 + rt;
         const int qh = head * a.group + rh;
-        const int own_chunks = attn8_chunks(a, last);
-        if (own_chunks <= 1) {
+        if constexpr (CL) {
+            store8(&s_co[r][d], true, f);
+            if (d == 0) { s_cm[r] = m; s_cl[r] = l; }
+        } else if (attn8_chunks(a, last) <= 1) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
             for (int k = 0; k < 8; ++k) f[k] *= inv;
@@ -475,52 +504,98 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
             if (d == 0) { a.part_ml[pi * 2] = m; a.part_ml[pi * 2 + 1] = l; }
         }
     }
+    if constexpr (CL) {
+    // The blocks' states, in their order: each block joins its share of the tile's values.
+    cluster_barrier();
+    for (int x = chunk * kA8Threads + tid; x < kA8Rows * HD / 4; x += a.n_chunks * kA8Threads) {
+        const int r = x / (HD / 4), d = (x % (HD / 4)) * 4;
+        const int rt = r / a.rows_heads, rh = ht * a.rows_heads + r % a.rows_heads;
+        if (rt >= n || rh >= a.group) continue;
+        float mp[kA8MaxCluster], lp[kA8MaxCluster], m = -INFINITY;
+        float4 v[kA8MaxCluster];
+#pragma unroll
+        for (int c = 0; c < kA8MaxCluster; ++c)
+            if (c < a.n_chunks) { mp[c] = peer_f32(&s_cm[r], c); lp[c] = peer_f32(&s_cl[r], c); v[c] = peer_f32x4(&s_co[r][d], c); }
+#pragma unroll
+        for (int c = 0; c < kA8MaxCluster; ++c)
+            if (c < a.n_chunks) m = fmaxf(m, mp[c]);
+        float l = 0.f, f[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kA8MaxCluster; ++c)
+            if (c < a.n_chunks) {
+                const float wt = part_weight(mp[c], lp[c], m);
+                if (wt == 0.f && lp[c] == 0.f) continue;
+                l += wt * lp[c];
+                f[0] += wt * v[c].x; f[1] += wt * v[c].y; f[2] += wt * v[c].z; f[3] += wt * v[c].w;
+            }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        T* dst = static_cast<T*>(a.out) + (long long)(t0 + rt) * a.out_stride + (head * a.group + rh) * HD + d;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) dst[k] = from_float<T>(f[k] * inv);
+    }
+    cluster_barrier();                                           // nobody's shared memory goes while it is read
+    }
 }
 
-// Joins the chunks of each (token, head), in their order: one warp each.  A row whose tile had one chunk is written already;
+// Joins the chunks of each (token, head), in their order: one block each.  A row whose tile had one chunk is written already;
 // a tile's chunks are those of its last row, so a row may have chunks in which it attends nothing (m = -inf, l = 0).
+// Bound by latency: all maxima in one round trip, all partial sums in another.
+constexpr int kA8MaxChunks = 1024;
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) k_attn_kv8_join(const Attn8Args a) {
+    constexpr int LANES = HD / 4, GROUPS = 128 / LANES;          // a thread has four dims of every GROUPS-th chunk
+    __shared__ float s_w[kA8MaxChunks], s_red[2][4], s_o[GROUPS][HD];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
-    const long long x = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (x >= (long long)a.n_tok * a.n_heads) return;
+    const long long x = blockIdx.x;
     const int tok = (int)(x / a.n_heads), qh = (int)(x % a.n_heads);
     const int seq = a.tok_seq[tok];
     if (seq < 0 || seq >= a.n_seq) return;
-    int last = tok;                                              // the tile's last token
+    int first = tok, last = tok;                                 // the tile's tokens
     if (a.cu_tok) {
-        const int first = a.cu_tok[seq], end = min(a.cu_tok[seq + 1], a.n_tok);
-        if (tok < first || tok >= end) return;                   // the lists contradict one another: no tile had this row
-        last = min(first + (tok - first) / a.rows_toks * a.rows_toks + a.rows_toks, end) - 1;
+        const int c0 = a.cu_tok[seq], end = min(a.cu_tok[seq + 1], a.n_tok);
+        if (tok < c0 || tok >= end) return;                      // the lists contradict one another: no tile had this row
+        first = c0 + (tok - c0) / a.rows_toks * a.rows_toks;
+        last = min(first + a.rows_toks, end) - 1;
     }
     int lp = -1;
-    for (int i = a.cu_tok ? a.cu_tok[seq] + (tok - a.cu_tok[seq]) / a.rows_toks * a.rows_toks : tok; i <= last; ++i) lp = max(lp, a.tok_pos[i]);
+    for (int i = first; i <= last; ++i) lp = max(lp, a.tok_pos[i]);
     lp = (int)min((long long)lp, (long long)a.width * kPage - 1);
     const int chunks = attn8_chunks(a, lp);
     if (chunks <= 1) return;
     const long long p0 = x * a.n_chunks;
     float m = -INFINITY;
-    for (int c = lane; c < chunks; c += 32) m = fmaxf(m, a.part_ml[(p0 + c) * 2]);
+    for (int c = tid; c < chunks; c += 128) { const float mc = a.part_ml[(p0 + c) * 2]; s_w[c] = mc; m = fmaxf(m, mc); }
     m = warp_max(m);
-    constexpr int DL = HD >= 32 ? HD / 32 : 1;
-    float l = 0.f, f[DL];
-#pragma unroll
-    for (int k = 0; k < DL; ++k) f[k] = 0.f;
-    for (int c = 0; c < chunks; ++c) {
-        const float mc = a.part_ml[(p0 + c) * 2], lc = a.part_ml[(p0 + c) * 2 + 1];
-        const float wt = mc == -INFINITY ? (lc == 0.f ? 0.f : 1.f) : exp2_fast(mc - m);
-        if (wt == 0.f && lc == 0.f) continue;
-        l += wt * lc;
-        if (lane * DL < HD)
-#pragma unroll
-            for (int k = 0; k < DL; ++k) f[k] += wt * a.part[(p0 + c) * HD + lane * DL + k];
+    if (lane == 0) s_red[0][warp] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+    float l = 0.f;
+    for (int c = tid; c < chunks; c += 128) {
+        const float mc = s_w[c], lc = a.part_ml[(p0 + c) * 2 + 1];
+        const float w = part_weight(mc, lc, m);
+        s_w[c] = w;
+        l += w == 0.f && lc == 0.f ? 0.f : w * lc;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (lane * DL < HD) {
-        T* dst = static_cast<T*>(a.out) + (long long)tok * a.out_stride + qh * HD + lane * DL;
+    l = warp_sum(l);
+    if (lane == 0) s_red[1][warp] = l;
+    __syncthreads();
+    l = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+    const int group = tid / LANES, d = (tid % LANES) * 4;
+    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = group; c < chunks; c += GROUPS) {
+        const float w = s_w[c];
+        const float4 v = *reinterpret_cast<const float4*>(a.part + (p0 + c) * HD + d);
+        f.x += w * v.x; f.y += w * v.y; f.z += w * v.z; f.w += w * v.w;
+    }
+    *reinterpret_cast<float4*>(&s_o[group][d]) = f;
+    __syncthreads();
+    if (tid < HD) {
+        float o = 0.f;
 #pragma unroll
-        for (int k = 0; k < DL; ++k) dst[k] = from_float<T>(f[k] * inv);
+        for (int k = 0; k < GROUPS; ++k) o += s_o[k][tid];
+        static_cast<T*>(a.out)[(long long)tok * a.out_stride + qh * HD + tid] = from_float<T>(l == 0.f ? 0.f : o / l);
     }
 }
 

@@ -73,15 +73,21 @@ Kv8View view(const sllm_kv8_layer* c) { return Kv8View{c->pages, c->scales, (lon
 
 // Every kernel here starts with griddepcontrol.wait, so it may be scheduled while the stream's previous kernel drains.
 template <typename... K, typename... A>
-int launch(const char* what, void (*kern)(K...), dim3 grid, int block, size_t smem, void* stream, A... args) {
+int launch_cluster(const char* what, void (*kern)(K...), dim3 grid, int block, size_t smem, void* stream, unsigned cluster_z, A... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid; cfg.blockDim = dim3(block); cfg.dynamicSmemBytes = smem; cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = cluster_z;
+    cfg.attrs = attr; cfg.numAttrs = cluster_z > 1 ? 2 : 1;
     if (cudaError_t err = cudaLaunchKernelEx(&cfg, kern, args...)) { (void)cudaGetLastError(); return cuda_fail(err, what); }
     return SLLM_OK;
+}
+template <typename... K, typename... A>
+int launch(const char* what, void (*kern)(K...), dim3 grid, int block, size_t smem, void* stream, A... args) {
+    return launch_cluster(what, kern, grid, block, smem, stream, 1, args...);
 }
 // Shared memory above 48 KB, asked for once per kernel and device.
 template <typename K>
@@ -157,20 +163,27 @@ Plan plan_attn(const sllm_kv8_layer* c, const sllm_kv8_attn* s, int sms) {
         a.n_chunks = 1;
         return p;
     }
-    // chunks of the keys: until there are two rounds of blocks, and none shorter than one unit per warp
+    // Chunks of the keys until there are about two rounds of blocks, none shorter than a unit per warp nor longer than 4096 keys (of
+    // rows of very different lengths; four documents of 60 to 131 thousand keys: 149 us without that, 132 with).  Few short rows are
+    // cut into at most eight, which a cluster joins: 6.9 us for ten heads of 2048 keys, where sixteen chunks and a second kernel
+    // take 7.6; with more blocks than two or three per SM the cluster's blocks wait for one another (16 sequences: 21 us, 14 without).
     const long long most = (long long)s->table_width * kPage, len = s->max_len ? std::min<long long>(s->max_len, most) : most;
     const long long base = (long long)p.tiles * c->kv_heads * a.head_tiles;
-    const long long want = 2ll * sms * (c->head_dim > 64 ? 2 : 4);
-    constexpr long long least = kA8Warps * kA8Unit;
-    long long chunks = std::max(1ll, std::min((want + base - 1) / base, (len + least - 1) / least));
+    const long long want = 2ll * sms * (c->head_dim > 64 ? 3 : 4);
+    constexpr long long least = kA8Warps * kA8Unit, longest = 4096;
+    long long chunks = std::max((want + base - 1) / base, base < want ? (len + longest - 1) / longest : 1ll);
+    chunks = std::max(1ll, std::min({chunks, (len + least - 1) / least, (long long)kA8MaxChunks}));
+    const bool few = len <= 2 * least * kA8MaxCluster && base * std::min<long long>(chunks, kA8MaxCluster) <= 5ll * sms / 2;
+    if (few) chunks = std::min<long long>(chunks, kA8MaxCluster);
     long long chunk = (len + chunks - 1) / chunks;
     chunk = (chunk + least - 1) / least * least;
     a.chunk = (int)chunk;
     a.n_chunks = (int)std::max(1ll, (len + chunk - 1) / chunk);
+    a.cluster = few && a.n_chunks > 1;
     return p;
 }
 uint64_t plan_bytes(const Plan& p, uint32_t hd) {
-    return p.a.n_chunks > 1 ? (uint64_t)p.a.n_tok * p.a.n_heads * p.a.n_chunks * (hd + 2) * sizeof(float) : 0;
+    return p.a.n_chunks > 1 && !p.a.cluster ? (uint64_t)p.a.n_tok * p.a.n_heads * p.a.n_chunks * (hd + 2) * sizeof(float) : 0;
 }
 
 int check_attn(const char* what, const sllm_kv8_layer* c, const sllm_kv8_attn* a) {
@@ -194,23 +207,25 @@ int check_attn(const char* what, const sllm_kv8_layer* c, const sllm_kv8_attn* a
     return SLLM_OK;
 }
 
-template <typename T, int HD, bool I8>
+template <typename T, int HD, bool I8, bool CL>
 int attn_form(const Plan& p, int dev, void* stream) {
     static std::atomic<uint64_t> done{0};
     const char* what = "sllm_k_attn_kv8";
-    if (int rc = opt_in(what, k_attn_kv8<T, HD, I8>, attn8_smem<HD>(), dev, done)) return rc;
+    if (int rc = opt_in(what, k_attn_kv8<T, HD, I8, CL>, attn8_smem<HD>(), dev, done)) return rc;
     const Attn8Args& a = p.a;
-    if (int rc = launch(what, k_attn_kv8<T, HD, I8>, dim3(p.tiles, a.c.H * a.head_tiles, a.n_chunks), kA8Threads, attn8_smem<HD>(), stream, a)) return rc;
-    if (a.n_chunks == 1) return SLLM_OK;
-    const long long pairs = (long long)a.n_tok * a.n_heads;
-    return launch(what, k_attn_kv8_join<T, HD>, dim3((unsigned)((pairs + 3) / 4)), 128, 0, stream, a);
+    const uint64_t blocks = (uint64_t)p.tiles * a.c.H * a.head_tiles, pairs = (uint64_t)a.n_tok * a.n_heads;
+    if (blocks > 0x7fffffffu || pairs > 0x7fffffffu) return bad(what, "too many rows and heads for one call");
+    const dim3 grid((unsigned)blocks, 1, a.n_chunks);
+    if (int rc = launch_cluster(what, k_attn_kv8<T, HD, I8, CL>, grid, kA8Threads, attn8_smem<HD>(), stream, CL ? a.n_chunks : 1, a)) return rc;
+    if (a.n_chunks == 1 || CL) return SLLM_OK;
+    return launch(what, k_attn_kv8_join<T, HD>, dim3((unsigned)pairs), 128, 0, stream, a);
 }
 template <typename T, int HD>
 int attn_hd(const Plan& p, int dev, void* stream) {
     // The integer form: bf16 rows, and no more keys per warp than its 32-bit sums hold whatever they are (2^17 products of 127 * 127).
     if constexpr (std::is_same<T, __nv_bfloat16>::value && HD >= 32)
-        if ((long long)p.a.width * kPage <= (long long)kA8Warps << 17) return attn_form<T, HD, true>(p, dev, stream);
-    return attn_form<T, HD, false>(p, dev, stream);
+        if ((long long)p.a.width * kPage <= (long long)kA8Warps << 17) return p.a.cluster ? attn_form<T, HD, true, true>(p, dev, stream) : attn_form<T, HD, true, false>(p, dev, stream);
+    return p.a.cluster ? attn_form<T, HD, false, true>(p, dev, stream) : attn_form<T, HD, false, false>(p, dev, stream);
 }
 template <int HD, int NT>
 int attn_tc(const Plan& p, int dev, void* stream) {
