@@ -107,7 +107,7 @@ int append_hd(const sllm_kv8_layer* c, const sllm_kv8_rows* r, int sms, void* st
     const unsigned windows = (r->n_tok + kAppendWindow - 1) / kAppendWindow;
     // A window has between 1 run (a prompt) and 16 (a decode step), 2 kv_heads units each.  Short lists get a warp for
     // every unit there could be; long ones one for each unit of a prompt's window.
-    const unsigned most = (2 * c->kv_heads * kAppendWindow + kAppendWarps - 1) / kAppendWarps, least = (2 * c->kv_heads + kAppendWarps - 1) / kAppendWarps;
+    const unsigned teams = kAppendWarps / (HD / 128 + 1), most = (2 * c->kv_heads * kAppendWindow + teams - 1) / teams, least = (2 * c->kv_heads + teams - 1) / teams;
     const unsigned y = std::min(most, std::max(least, (unsigned)(sms * 16) / windows));
     return launch("sllm_k_kv8_append", k_kv8_append<T, HD>, dim3(windows, y), kAppendWarps * 32, 0, stream, a);
 }
@@ -118,6 +118,21 @@ int append_t(const sllm_kv8_layer* c, const sllm_kv8_rows* r, int sms, void* str
         case 32: return append_hd<T, 32>(c, r, sms, stream);
         case 64: return append_hd<T, 64>(c, r, sms, stream);
         default: return append_hd<T, 128>(c, r, sms, stream);
+    }
+}
+
+template <typename T, int HD>
+int read_hd(const sllm_kv8_layer* c, const Read8Args& a, void* stream) {
+    constexpr int rows = kReadThreads / (HD / 8) * 4;
+    return launch("sllm_k_kv8_read", k_kv8_read<T, HD>, dim3((a.n_tok + rows - 1) / rows, 2 * c->kv_heads), kReadThreads, 0, stream, a);
+}
+template <typename T>
+int read_t(const sllm_kv8_layer* c, const Read8Args& a, void* stream) {
+    switch (c->head_dim) {
+        case 16: return read_hd<T, 16>(c, a, stream);
+        case 32: return read_hd<T, 32>(c, a, stream);
+        case 64: return read_hd<T, 64>(c, a, stream);
+        default: return read_hd<T, 128>(c, a, stream);
     }
 }
 
@@ -286,11 +301,9 @@ int sllm_k_kv8_read(const sllm_kv8_layer* c, const sllm_kv8_rows* r, void* strea
     if (r->n_tok == 0) return SLLM_OK;
     const size_t w = r->dtype == SLLM_ROWS_BF16 ? 2 : 4;
     Read8Args a{view(c), const_cast<void*>(r->k), const_cast<void*>(r->v), reinterpret_cast<const long long*>(r->slot_map), (long long)r->k_stride, (long long)r->v_stride,
-                (int)r->n_tok, (int)c->head_dim, 0};
+                (int)r->n_tok, 0};
     a.wide = aligned(r->k, 16) && aligned(r->v, 16) && (r->k_stride * w) % 16 == 0 && (r->v_stride * w) % 16 == 0;
-    const long long items = (long long)r->n_tok * c->kv_heads * 2 * (c->head_dim / 8);
-    const unsigned grid = (unsigned)std::min<long long>((items + 255) / 256, (long long)sms * 64);
-    return r->dtype == SLLM_ROWS_F32 ? launch(what, k_kv8_read<float>, dim3(grid), 256, 0, stream, a) : launch(what, k_kv8_read<__nv_bfloat16>, dim3(grid), 256, 0, stream, a);
+    return r->dtype == SLLM_ROWS_F32 ? read_t<float>(c, a, stream) : read_t<__nv_bfloat16>(c, a, stream);
 }
 
 int sllm_k_attn_kv8_workspace(const sllm_kv8_layer* c, const sllm_kv8_attn* s, uint64_t* bytes) {

@@ -185,15 +185,30 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, bool wide, const float*
     }
 }
 
-// rint(x / s), ties to even, as if the quotient were exact.  x * (1 / s) is within one integer of it; the remainder
-// x - q s is exact in one fma (|q| <= 127, and it is at most about s / 2, so its bits fit), which settles the rest.
-__device__ __forceinline__ int quant8(float x, float s, float inv) {
-    float q = rintf(x * inv);
-    const float r = fmaf(-q, s, x), half = 0.5f * s;
-    const int qi = (int)q;
-    if (r > half || (r == half && (qi & 1))) return qi + 1;
-    if (r < -half || (r == -half && (qi & 1))) return qi - 1;
-    return qi;
+// Eight values' rint(x / s), ties to even, as if the quotients were exact, as bytes.  x * (1 / s) rounded to an integer (by the
+// addition of 1.5 * 2^23, which costs no conversion) is within one of it; the remainder x - q s is exact in one fma (|q| <= 127, and it is
+// at most about s / 2, so its bits fit) and settles the rest, which is looked at only where it reaches s / 2.
+__device__ __forceinline__ uint2 quant8(const float* x, float s, float inv) {
+    constexpr float kBias = 12582912.f;
+    uint32_t b[8];
+    float r[8], worst = 0.f;
+    const float half = 0.5f * s;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float y = fmaf(x[j], inv, kBias), q = y - kBias;
+        b[j] = __float_as_uint(y);
+        r[j] = fmaf(-q, s, x[j]);
+        worst = fmaxf(worst, fabsf(r[j]));
+    }
+    if (worst >= half) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (r[j] > half || (r[j] == half && (b[j] & 1))) b[j] += 1;
+            else if (r[j] < -half || (r[j] == -half && (b[j] & 1))) b[j] -= 1;
+        }
+    }
+    const uint32_t b01 = __byte_perm(b[0], b[1], 0x0040), b23 = __byte_perm(b[2], b[3], 0x0040), b45 = __byte_perm(b[4], b[5], 0x0040), b67 = __byte_perm(b[6], b[7], 0x0040);
+    return make_uint2(__byte_perm(b01, b23, 0x5410), __byte_perm(b45, b67, 0x5410));
 }
 
 // ---- append -------------------------------------------------------------------------------------------------------
@@ -216,12 +231,15 @@ constexpr int kAppendWindow = 16;      // list entries whose leaders one block h
 // it, and goes when the block is started anew.  The smallest scale of a block with anything in it is 2^-126, so that 1 / s
 // is finite.
 // A block of threads takes the leaders among 16 list entries (31 slots say where their runs end).  The rows are read once and
-// kept in registers between the maximum and the rounding; bound by the bytes of long lists, by latency in short ones.
+// kept in registers between the maximum and the rounding; at head_dim 128 two warps share a block of 16 rows, so that four
+// blocks of threads and not two fit an SM.  Bound by the bytes of long lists and the round trips to them, by latency in short ones.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kAppendWarps * 32) k_kv8_append(const Append8Args a) {
     constexpr int VPR = HD / 8;                         // vectors of 8 per row
-    constexpr int VPL = (kBlk8 * VPR + 31) / 32;        // vectors per lane and block
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int W = HD / 128 + 1, TEAM = W * 32;      // warps, threads of a unit
+    constexpr int VPL = (kBlk8 * VPR + TEAM - 1) / TEAM;        // vectors per thread and unit
+    __shared__ unsigned s_top[2][kAppendWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, team = warp / W, member = threadIdx.x % TEAM;
     const int t0 = blockIdx.x * kAppendWindow;
     pdl_wait();
     // lane l: slot of entry t0 - 1 + l
@@ -237,7 +255,8 @@ __global__ void __launch_bounds__(kAppendWarps * 32) k_kv8_append(const Append8A
     const unsigned follow_mask = __ballot_sync(0xffffffffu, follows);
     const unsigned leaders = __ballot_sync(0xffffffffu, live && !follows && lane >= 1 && lane <= kAppendWindow);
     const int units = __popc(leaders) * a.c.H * 2;
-    for (int u = blockIdx.y * kAppendWarps + warp; u < units; u += gridDim.y * kAppendWarps) {
+    int odd = 0;
+    for (int u = blockIdx.y * (kAppendWarps / W) + team; u < units; u += gridDim.y * (kAppendWarps / W), odd ^= 1) {
         const int hw = u % (a.c.H * 2), head = hw >> 1, which = hw & 1;
         unsigned rest = leaders;
         for (int k = u / (a.c.H * 2); k > 0; --k) rest &= rest - 1;
@@ -256,7 +275,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) k_kv8_append(const Append8A
         unsigned top = 0;                                           // bits of the largest magnitude: NaN above infinity above all else
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-            const int e = i * 32 + lane, row = e / VPR;
+            const int e = i * TEAM + member, row = e / VPR;
             if (row < m) {
                 load8(src + (long long)(t0 - 1 + lead + row) * stride + head * HD + (e % VPR) * 8, a.wide, x[i]);
 #pragma unroll
@@ -264,6 +283,11 @@ __global__ void __launch_bounds__(kAppendWarps * 32) k_kv8_append(const Append8A
             }
         }
         top = __reduce_max_sync(0xffffffffu, top);
+        if (W > 1) {                                                // the unit's other warp; the next unit writes the other half of s_top
+            if (lane == 0) s_top[odd][warp] = top;
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(TEAM) : "memory");
+            top = max(top, s_top[odd][warp ^ 1]);
+        }
         float s = __fdiv_rn(__uint_as_float(top), 127.f);
         if (top) s = fmaxf(s, 1.17549435e-38f);
         const bool nan = top >= 0x7f800000u || s_old != s_old;
@@ -271,7 +295,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) k_kv8_append(const Append8A
         const float inv = s > 0.f ? __frcp_rn(s) : 0.f;             // also 0 for NaN: compares false
         if (off && !(s == s_old)) {
             const double so = s_old, sn = s;
-            for (int e = lane; e < off * VPR; e += 32) {
+            for (int e = member; e < off * VPR; e += TEAM) {
                 uint2 w = *reinterpret_cast<const uint2*>(dst + e * 8);
                 int8_t* q = reinterpret_cast<int8_t*>(&w);
 #pragma unroll
@@ -281,20 +305,10 @@ __global__ void __launch_bounds__(kAppendWarps * 32) k_kv8_append(const Append8A
         }
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-            const int e = i * 32 + lane, row = e / VPR;
-            if (row < m) {
-                uint2 w = make_uint2(0u, 0u);
-                if (!nan) {
-                    uint32_t b[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) b[j] = (uint32_t)quant8(x[i][j], s, inv) & 0xffu;
-                    w.x = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
-                    w.y = b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24;
-                }
-                *reinterpret_cast<uint2*>(dst + (off + row) * HD + (e % VPR) * 8) = w;
-            }
+            const int e = i * TEAM + member, row = e / VPR;
+            if (row < m) *reinterpret_cast<uint2*>(dst + (off + row) * HD + (e % VPR) * 8) = nan ? make_uint2(0u, 0u) : quant8(x[i], s, inv);
         }
-        if (lane == 0) *sc = s;
+        if (member == 0) *sc = s;
     }
 }
 
@@ -304,33 +318,50 @@ struct Read8Args {
     void* k; void* v;
     const long long* slots;
     long long k_stride, v_stride;
-    int n_tok, hd, wide;
+    int n_tok, wide;
 };
 
-// One thread per eight values: a row of K and of V per list entry, zeros for a slot outside the pool.  Bound by bytes
-// (1 in, 2 or 4 out per value).
-template <typename T>
-__global__ void __launch_bounds__(256) k_kv8_read(const Read8Args a) {
+// A block takes one head's K or V of kReadRows list entries, a thread eight values of four of them: rows of K and of V per
+// entry, zeros for a slot outside the pool.  Bound by bytes (1 in, 2 or 4 out per value).
+constexpr int kReadThreads = 256;
+template <typename T, int HD>
+__global__ void __launch_bounds__(kReadThreads) k_kv8_read(const Read8Args a) {
+    constexpr int VPR = HD / 8, RPP = kReadThreads / VPR;        // threads per row, rows per pass
     pdl_wait();
-    const int vpr = a.hd / 8;
-    const long long per = (long long)a.c.H * 2 * vpr;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.n_tok * per; i += (long long)gridDim.x * 256) {
-        const int t = (int)(i / per), r = (int)(i % per);
-        const int which = r / (a.c.H * vpr), hv = r % (a.c.H * vpr), head = hv / vpr, vec = hv % vpr;
-        const long long slot = a.slots[t];
-        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (slot >= 0 && slot < a.c.n_pages * kPage) {
-            const long long page = slot / kPage;
-            const int at = (int)(slot % kPage);
-            const long long run = (page * a.c.H + head) * 2 + which;
-            const float s = a.c.scales[run * kBlksPerPage + at / kBlk8];
-            const uint2 w = *reinterpret_cast<const uint2*>(a.c.pages + (run * kPage + at) * a.hd + vec * 8);
-            const int8_t* q = reinterpret_cast<const int8_t*>(&w);
+    const int head = blockIdx.y >> 1, which = blockIdx.y & 1, vec = threadIdx.x % VPR;
+    T* out = static_cast<T*>(which ? a.v : a.k) + head * HD + vec * 8;
+    const long long stride = which ? a.v_stride : a.k_stride;
+    const int t0 = blockIdx.x * RPP * 4 + threadIdx.x / VPR;
+    long long run[4];
+    int at[4];
+    uint2 w[4];
+    float s[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = (float)q[j] * s;
+    for (int i = 0; i < 4; ++i) {
+        const int t = t0 + i * RPP;
+        const long long slot = t < a.n_tok ? a.slots[t] : -1;
+        const bool in = slot >= 0 && slot < a.c.n_pages * kPage;
+        run[i] = in ? ((slot / kPage) * a.c.H + head) * 2 + which : -1;
+        at[i] = (int)(slot & (kPage - 1));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = make_uint2(0u, 0u); s[i] = 0.f;
+        if (run[i] >= 0) {
+            w[i] = *reinterpret_cast<const uint2*>(a.c.pages + (run[i] * kPage + at[i]) * HD + vec * 8);
+            s[i] = a.c.scales[run[i] * kBlksPerPage + at[i] / kBlk8];
         }
-        T* dst = static_cast<T*>(which ? a.v : a.k) + t * (which ? a.v_stride : a.k_stride) + hv * 8;
-        store8(dst, a.wide, f);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int t = t0 + i * RPP;
+        if (t >= a.n_tok) continue;
+        float f[8];
+        const uint32_t u[2] = {w[i].x ^ 0x80808080u, w[i].y ^ 0x80808080u};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)                              // a byte under 2^23: no conversion instruction
+            f[j] = (__uint_as_float(__byte_perm(u[j >> 2], 0x4b000000u, 0x7440 + (j & 3))) - 8388736.f) * s[i];
+        store8(out + t * stride, a.wide, f);
     }
 }
 

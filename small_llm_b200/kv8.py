@@ -145,7 +145,8 @@ def read(slots: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, dtype: 
     t, n = _ROWS.get(dtype), slots.shape[0]
     _need(t is not None, "dtype must be bfloat16 or float32")
     at = _flat("slots", slots, _I64, (n,), dev)
-    k, v = torch.empty((2, n, h, d), dtype=dtype, device=pages.device).unbind(0)
+    k = scales.new_empty((n, h, d), dtype=dtype)
+    v = torch.empty_like(k)
     if n:
         _call(dev, _lib().sllm_k_kv8_read, c, _pack_rows(k.data_ptr(), v.data_ptr(), at, h * d, h * d, n, t))
     return k, v
