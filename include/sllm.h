@@ -242,7 +242,7 @@ int sllm_k_attn_decode_static(sllm_engine* e, uint32_t layer, uint32_t n_tok, co
 /* One layer of the cache.  A slot is page * 64 + (position % 64). */
 typedef struct {
     int8_t* pages;             /* [n_pages][kv_heads][2][64][head_dim], [2]: K, V; 16-byte aligned                */
-    float* scales;             /* [n_pages][kv_heads][2][4], 16-byte aligned                                       */
+    float* scales;             /* [n_pages][kv_heads][2][4], 16-byte aligned; never negative                       */
     uint64_t n_pages;          /* 1 .. 2^31 - 1                                                                    */
     uint32_t kv_heads, head_dim;   /* head_dim 16, 32, 64 or 128                                                   */
 } sllm_kv8_layer;
@@ -272,7 +272,7 @@ typedef struct {
     int32_t *tok_seq, *tok_pos;               /* [max_tok]                                                         */
     int64_t* slot_map;                        /* [max_tok]                                                         */
     uint64_t n_pages;
-    uint32_t n_seq, table_width, max_tok;     /* n_seq 1 .. 8192                                                   */
+    uint32_t n_seq, table_width, max_tok;     /* n_seq 1 .. 8192, table_width 1 .. 2^24                            */
 } sllm_block_tables;
 int sllm_k_block_tables(const sllm_block_tables* a, void* stream);
 

@@ -149,7 +149,7 @@ __device__ __forceinline__ float4 peer_f32x4(const float* p, int rank) {
 // weight of a part with maximum mp and sum lp in a whole with maximum m: a part whose scores are all NaN has no maximum, but its sum says so
 __device__ __forceinline__ float part_weight(float mp, float lp, float m) { return mp == -INFINITY ? (lp == 0.f ? 0.f : 1.f) : exp2_fast(mp - m); }
 // chunks of a tile whose last row stands at `last`
-__device__ __forceinline__ int attn8_chunks(const Attn8Args& a, int last) { return min((last + a.chunk) / a.chunk, a.n_chunks); }
+__device__ __forceinline__ int attn8_chunks(const Attn8Args& a, int last) { return (int)min(((long long)last + a.chunk) / a.chunk, (long long)a.n_chunks); }
 
 // CL: the chunks of a tile are a cluster's blocks (a form of its own: it costs registers, and with them blocks per SM)
 template <typename T, int HD, bool I8, bool CL>

@@ -15,6 +15,7 @@
 // passed by more than 8 (a factor of 256, which fp16 and the fp32 sums take): O in tensor memory is then rescaled, which is rare.
 //
 // Bound by the exponentials (16 a clock and SM: 1024 clocks per 128 x 128 tile) and, at head_dim 128, equally by the products.
+// Where there are few blocks for the GPU the keys are cut into chunks (grid z), whose states the general form's second kernel joins.
 // Every wait is bounded; on expiry the block sets *status, frees its tensor memory and returns.
 #pragma once
 #include "attn_kv8.cuh"
@@ -169,6 +170,23 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
     const int head = blockIdx.x, group = a.group, toks = a.rows_toks / NT;   // tokens of one tile
     const int most = (int)min((long long)a.width * kPage, 0x7fffff00ll) - 1;
 
+    // last position of each tile's tokens
+    if (tid < 2 * kT8Rows) {
+        const int pos = tid < n ? min(a.tok_pos[t0 + tid], most) : -1;
+        const int p0 = __reduce_max_sync(0xffffffffu, tid < toks ? pos : -1), p1 = __reduce_max_sync(0xffffffffu, tid < toks ? -1 : pos);
+        if (lane == 0) { s_last[0][warp] = p0; s_last[1][warp] = p1; }
+    }
+    __syncthreads();
+    int last0 = -1, last1 = -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { last0 = max(last0, s_last[0][i]); last1 = max(last1, s_last[1][i]); }
+    // This block's chunk of the keys: from here on positions and pages count from its first key.  The last chunk takes all that is left.
+    const int chunk = blockIdx.z, key0 = chunk * a.chunk, own_chunks = attn8_chunks(a, max(last0, last1));
+    const int last = max(last0, last1) - key0, most_steps = chunk == a.n_chunks - 1 ? 0x7fffffff : a.chunk / kT8Keys;
+    const int n0 = min(max(last0 - key0 + kT8Keys, 0) / kT8Keys, most_steps), n1 = min(max(last1 - key0 + kT8Keys, 0) / kT8Keys, most_steps);
+    const int steps = max(n0, n1);                            // 0 where nothing is attended
+    if (steps == 0 && chunk > 0) return;                      // chunk 0 writes the rows that attend nothing
+
     if (tid == 0) {
         for (int i = 0; i < kT8Stages; ++i) { mbar_init(B(K_FULL + i), 5); mbar_init(B(V_FULL + i), 4); mbar_init(B(K_FREE + i), 1); mbar_init(B(V_FREE + i), 1); }
         for (int i = 0; i < 4; ++i) { mbar_init(B(S_READY + i), 1); mbar_init(B(P_READY + i), 4); mbar_init(B(PV_DONE + i), 1); }
@@ -181,24 +199,13 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
 
-    // last position of each tile's tokens
-    if (tid < 2 * kT8Rows) {
-        const int pos = tid < n ? min(a.tok_pos[t0 + tid], most) : -1;
-        const int p0 = __reduce_max_sync(0xffffffffu, tid < toks ? pos : -1), p1 = __reduce_max_sync(0xffffffffu, tid < toks ? -1 : pos);
-        if (lane == 0) { s_last[0][warp] = p0; s_last[1][warp] = p1; }
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    int last0 = -1, last1 = -1;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { last0 = max(last0, s_last[0][i]); last1 = max(last1, s_last[1][i]); }
-    const int last = max(last0, last1);
-    const int n0 = (last0 + kT8Keys) / kT8Keys, n1 = (last1 + kT8Keys) / kT8Keys, steps = max(n0, n1);     // 0 where nothing is attended
     bool ok = true;
 
-    const int* table = a.table + (size_t)seq * a.width;
+    const int* table = a.table + (size_t)seq * a.width + key0 / kPage;
     auto page_of = [&](int i) -> int {                        // page of a step; -2: outside the pool
         const int id = table[i];
         return id < 0 || id >= a.c.n_pages ? -2 : id;
@@ -368,7 +375,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
             const int rt = tile * toks + r / group;
             const bool valid = r / group < toks && rt < n;
             if (valid) { row_tok = t0 + rt; row_head = head * group + r % group; }
-            pos = valid ? min(a.tok_pos[row_tok], most) : -1;
+            pos = valid ? min(a.tok_pos[row_tok], most) - key0 : -1;
             uint4 raw[HD / 8];
             const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + (valid ? (long long)row_tok * a.q_stride + row_head * HD : 0);
             unsigned top = 0;
@@ -517,16 +524,21 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
         if (ok) {
-            const float inv = l == 0.f ? 0.f : vr / l;
+            const bool whole = own_chunks <= 1;
+            const float f = whole ? (l == 0.f ? 0.f : vr / l) : vr;
+            const long long part = ((long long)row_tok * a.n_heads + row_head) * a.n_chunks + chunk;
             __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (row_tok >= 0 ? (long long)row_tok * a.out_stride + row_head * HD : 0);
+            if (!whole && row_tok >= 0) { a.part_ml[part * 2] = m; a.part_ml[part * 2 + 1] = l; }
 #pragma unroll
             for (int h = 0; h < HD / 16; ++h) {
                 uint32_t o[16];
                 if (my_steps > 0) tc_ld16(o_at + h * 16, o);
                 float x[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] = l == 0.f || my_steps == 0 ? 0.f : __uint_as_float(o[j]) * inv;
-                if (row_tok >= 0) { store8(dst + h * 16, a.wide, x); store8(dst + h * 16 + 8, a.wide, x + 8); }
+                for (int j = 0; j < 16; ++j) x[j] = l == 0.f || my_steps == 0 ? 0.f : __uint_as_float(o[j]) * f;
+                if (row_tok < 0) continue;
+                if (whole) { store8(dst + h * 16, a.wide, x); store8(dst + h * 16 + 8, a.wide, x + 8); }
+                else { store8(a.part + part * HD + h * 16, true, x); store8(a.part + part * HD + h * 16 + 8, true, x + 8); }
             }
         }
     }

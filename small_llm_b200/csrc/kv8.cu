@@ -169,20 +169,31 @@ Plan plan_attn(const sllm_kv8_layer* c, const sllm_kv8_attn* s, int sms) {
     a.wide = aligned(s->q, 16) && aligned(s->out, 16) && (s->q_stride * w) % 16 == 0 && (s->out_stride * w) % 16 == 0;
     a.scale = s->scale != 0.f ? s->scale : 1.0f / std::sqrt((float)c->head_dim);
     a.status = s->status;
-    // Runs of many rows take the tensor-core form.
-    const long long run = s->max_new ? s->max_new : s->n_tok;
-    p.tc = a.cu_tok && s->dtype == SLLM_ROWS_BF16 && c->head_dim >= 64 && a.group <= kT8Rows && run * a.group >= 64 && s->n_tok / (kT8Rows / a.group) + (uint64_t)s->n_seq <= 65535;
+    // bf16 rows of runs of many (tokens x heads of a group) take the tensor-core form, whose tiles of 128 rows cost the same whatever
+    // part of them is filled.  Ten heads of 64, us there and in the general form: 64 sequences of 1 to 64 new tokens (32 rows on
+    // average) 87 and 71, 16 of 16 to 80 (48 rows) 30 and 43, 4 of 200 17 and 37.
+    p.tc = a.cu_tok && s->dtype == SLLM_ROWS_BF16 && c->head_dim >= 64 && a.group <= kT8Rows && (uint64_t)s->n_tok * a.group >= 40ull * s->n_seq &&
+           s->n_tok / (kT8Rows / a.group) + (uint64_t)s->n_seq <= 65535;
+    const long long most = (long long)s->table_width * kPage, len = s->max_len ? std::min<long long>(s->max_len, most) : most;
     if (p.tc) {
-        a.rows_toks = (c->head_dim == 64 ? 1 : 2) * (kT8Rows / a.group);
+        // Two tiles of query rows per block share the widening of K and V, which pays at head_dim 128 (in small grids too: 300 tokens of
+        // 4 sequences 60 us either way, 2000 of one 64 us against 74); at 64 one leaves two blocks to an SM, which hides a block's
+        // beginning and end.
+        const int nt = c->head_dim == 64 ? 1 : 2;
+        a.rows_toks = nt * (kT8Rows / a.group);
         p.tiles = s->n_tok / a.rows_toks + s->n_seq;
-        a.n_chunks = 1;
+        // Chunks, of at least 1024 keys, only where the blocks would not fill half the GPU: their states are fp32 rows in the workspace
+        // (a step with 3100 tokens in three chunks 108 us, uncut 77).
+        const long long base = (long long)p.tiles * c->kv_heads, slots = (nt == 1 ? 2ll : 1ll) * sms;
+        const long long chunks = std::max(1ll, std::min(slots / base, len / 1024));
+        a.chunk = (int)((len + chunks * kPage - 1) / (chunks * kPage)) * kPage;
+        a.n_chunks = (int)std::max(1ll, (len + a.chunk - 1) / a.chunk);
         return p;
     }
     // Chunks of the keys until there are about two rounds of blocks, none shorter than a unit per warp nor longer than 4096 keys (of
     // rows of very different lengths; four documents of 60 to 131 thousand keys: 149 us without that, 132 with).  Few short rows are
     // cut into at most eight, which a cluster joins: 6.9 us for ten heads of 2048 keys, where sixteen chunks and a second kernel
     // take 7.6; with more blocks than two or three per SM the cluster's blocks wait for one another (16 sequences: 21 us, 14 without).
-    const long long most = (long long)s->table_width * kPage, len = s->max_len ? std::min<long long>(s->max_len, most) : most;
     const long long base = (long long)p.tiles * c->kv_heads * a.head_tiles;
     const long long want = 2ll * sms * (c->head_dim > 64 ? 3 : 4);
     constexpr long long least = kA8Warps * kA8Unit, longest = 4096;
@@ -207,7 +218,7 @@ int check_attn(const char* what, const sllm_kv8_layer* c, const sllm_kv8_attn* a
     if (a->dtype != SLLM_ROWS_BF16 && a->dtype != SLLM_ROWS_F32) return bad(what, "dtype must be SLLM_ROWS_BF16 or SLLM_ROWS_F32");
     if (a->n_heads < 1 || a->n_heads % c->kv_heads != 0 || a->n_heads > 65535) return bad(what, "n_heads must be a multiple of kv_heads");
     if (a->n_seq < 1 || a->n_seq > 0x1000000u || a->n_tok > 0x1000000u) return bad(what, "n_seq must be 1..2^24, n_tok at most 2^24");
-    if (a->table_width < 1 || a->table_width > 0x1ffffffu) return bad(what, "table_width must be 1..2^25 - 1");
+    if (a->table_width < 1 || a->table_width > 0x1000000u) return bad(what, "table_width must be 1..2^24");
     const uint64_t row = (uint64_t)a->n_heads * c->head_dim;
     if (a->q_stride < row || a->out_stride < row || a->q_stride >> 40 || a->out_stride >> 40) return bad(what, "a row stride is shorter than n_heads * head_dim, or absurd");
     const size_t w = a->dtype == SLLM_ROWS_BF16 ? 2 : 4;
@@ -222,18 +233,22 @@ int check_attn(const char* what, const sllm_kv8_layer* c, const sllm_kv8_attn* a
     return SLLM_OK;
 }
 
+template <typename T, int HD>
+int join_chunks(const Attn8Args& a, void* stream) {
+    return launch("sllm_k_attn_kv8", k_attn_kv8_join<T, HD>, dim3((unsigned)a.n_tok * a.n_heads), 128, 0, stream, a);
+}
 template <typename T, int HD, bool I8, bool CL>
 int attn_form(const Plan& p, int dev, void* stream) {
     static std::atomic<uint64_t> done{0};
     const char* what = "sllm_k_attn_kv8";
     if (int rc = opt_in(what, k_attn_kv8<T, HD, I8, CL>, attn8_smem<HD>(), dev, done)) return rc;
     const Attn8Args& a = p.a;
-    const uint64_t blocks = (uint64_t)p.tiles * a.c.H * a.head_tiles, pairs = (uint64_t)a.n_tok * a.n_heads;
-    if (blocks > 0x7fffffffu || pairs > 0x7fffffffu) return bad(what, "too many rows and heads for one call");
+    const uint64_t blocks = (uint64_t)p.tiles * a.c.H * a.head_tiles;
+    if (blocks > 0x7fffffffu) return bad(what, "too many rows and heads for one call");
     const dim3 grid((unsigned)blocks, 1, a.n_chunks);
     if (int rc = launch_cluster(what, k_attn_kv8<T, HD, I8, CL>, grid, kA8Threads, attn8_smem<HD>(), stream, CL ? a.n_chunks : 1, a)) return rc;
     if (a.n_chunks == 1 || CL) return SLLM_OK;
-    return launch(what, k_attn_kv8_join<T, HD>, dim3((unsigned)pairs), 128, 0, stream, a);
+    return join_chunks<T, HD>(a, stream);
 }
 template <typename T, int HD>
 int attn_hd(const Plan& p, int dev, void* stream) {
@@ -247,7 +262,8 @@ int attn_tc(const Plan& p, int dev, void* stream) {
     static std::atomic<uint64_t> done{0};
     const char* what = "sllm_k_attn_kv8";
     if (int rc = opt_in(what, k_attn_kv8_tc<HD, NT>, attn8_tc_smem<HD, NT>(), dev, done)) return rc;
-    return launch(what, k_attn_kv8_tc<HD, NT>, dim3(p.a.c.H, p.tiles), attn8_tc_threads<NT>(), attn8_tc_smem<HD, NT>(), stream, p.a);
+    if (int rc = launch(what, k_attn_kv8_tc<HD, NT>, dim3(p.a.c.H, p.tiles, p.a.n_chunks), attn8_tc_threads<NT>(), attn8_tc_smem<HD, NT>(), stream, p.a)) return rc;
+    return p.a.n_chunks == 1 ? SLLM_OK : join_chunks<__nv_bfloat16, HD>(p.a, stream);
 }
 template <typename T>
 int attn_t(const Plan& p, uint32_t hd, int dev, void* stream) {
@@ -268,7 +284,7 @@ int sllm_k_block_tables(const sllm_block_tables* s, void* stream) {
     if (!s || !s->len_before || !s->len_after || !s->table || !s->ring || !s->pool_in || !s->pool_out || !s->cu_tok || !s->tok_seq || !s->tok_pos || !s->slot_map)
         return bad(what, "null pointer");
     if (s->n_seq < 1 || s->n_seq > (uint32_t)kTablesMaxSeq) return bad(what, "n_seq must be 1..8192");
-    if (s->table_width < 1 || s->table_width > 0x1ffffffu) return bad(what, "table_width must be 1..2^25 - 1");
+    if (s->table_width < 1 || s->table_width > 0x1000000u) return bad(what, "table_width must be 1..2^24");
     if (s->n_pages < 1 || s->n_pages > 0x7fffffffull) return bad(what, "n_pages must be 1..2^31 - 1");
     if (s->max_tok > 0x40000000u) return bad(what, "max_tok is too large");
     if (s->pool_in < s->pool_out + 4 && s->pool_out < s->pool_in + 4) return bad(what, "pool_in and pool_out overlap");
@@ -324,6 +340,7 @@ int sllm_k_attn_kv8(const sllm_kv8_layer* c, const sllm_kv8_attn* s, void* works
     if (int rc = check_memory(what, dev, {c->pages, c->scales, s->q, s->out, s->table, s->tok_seq, s->tok_pos, s->cu_tok, s->status, workspace})) return rc;
     if (s->n_tok == 0) return SLLM_OK;
     Plan p = plan_attn(c, s, sms);
+    if ((uint64_t)s->n_tok * s->n_heads > 0x7fffffffu) return bad(what, "too many rows and heads for one call");
     const uint64_t need = plan_bytes(p, c->head_dim);
     if (need) {
         if (!workspace || workspace_bytes < need || !aligned(workspace, 16))

@@ -379,6 +379,21 @@ def test_long_prompts(h, grp, d):
     check_attention(b, torch.bfloat16, max_new=90, max_len=3090, cu_tok=b[6], scale=-0.2)
 
 
+@pytest.mark.parametrize("h,grp,d", [(1, 1, 64), (2, 4, 128), (1, 3, 64)])
+def test_prompts_behind_long_histories_in_chunks(h, grp, d):
+    """Few query rows and many keys: the keys of a tile in chunks, of which short sequences have one and some rows attend none."""
+    a = setup_attention([9000, 3, 2500, 1023, 1024], [70, 64, 130, 1, 66], h, grp, d, torch.bfloat16, seed=d + 3 * grp, extra_rows=2)
+    for max_len in (9070, 0, 1500):
+        check_attention(a, torch.bfloat16, max_new=130, max_len=max_len, cu_tok=a[6])
+    q, pages, scales, table, seq, pos, cu = a
+    pos[3], pos[10], pos[80] = -1, 20, -1
+    scales[int(table[0, 30]), 0, 0, 1] = math.nan                            # shows from its first key on
+    got = kv8.attention(q, pages, scales, table, seq, pos, cu, max_new=130, max_len=9070, out=torch.zeros_like(q))
+    bad = torch.isnan(got).any(-1)[:, :grp].all(1).cpu()
+    assert bad.tolist() == [i < 70 and i not in (3, 10) for i in range(len(seq))]
+    assert float(got[3].abs().max()) == 0.0 and float(got[80].abs().max()) == 0.0
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("order", [1, -1])
 def test_prompts_with_scales_of_many_magnitudes(d, order):
