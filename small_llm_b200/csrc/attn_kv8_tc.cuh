@@ -1,20 +1,29 @@
 // Attention over the 8-bit paged cache (kv8.cuh) for prompts: bf16 rows, head_dim 64 or 128, on the 5th-generation tensor cores.
 //
-// One block takes one kv head and two tiles of 128 query rows (tokens x heads of the group) that follow on one another, so
-// that a key is widened once for 256 rows.  Per step of 128 keys (two pages):
+// One block takes one kv head and NT tiles of 128 query rows (tokens x heads of the group) that follow on one another: two at
+// head_dim 128, so that a key is widened once for 256 rows; one at 64, which leaves two blocks to an SM.  Per step, a page of 64 keys:
 //   widening warps   int8 K and V from global memory (a step ahead, in registers) -> fp16 in shared memory, 128-byte swizzle
-//   MMA warp         S_t = Q_t K^T, 128 x 128 x hd;  O_t += P_t V, 128 x hd x 128, accumulated in tensor memory   (t = 0, 1)
+//   scales' warp     the four blocks' factors
+//   MMA warp         S_t = Q_t K^T, 128 x 64 x hd, two steps ahead of the softmax, into one of two buffers;
+//                    O_t += P_t V, 128 x hd x 64; both in tensor memory
 //   softmax t        thread = query row = TMEM lane: w = exp2(...) as fp16 over S_t's own columns, where the next product reads it
-// While one tile's softmax runs, the tensor cores work on the other's products.
 //
 // The integers are multiplied as they are (exact in fp16), scales act outside the products and cost nothing per element: with
 // c = scale log2(e) ks(block) and v = vs(block) / vr the weight is  w = p v = exp2(S c + (log2 v - m)),  one fma and one ex2, and
 // the softmax denominator sums w / v block by block.  vr, a power of two no smaller than any vs so far, keeps w in fp16's range.
 // w is rounded to fp16 (2^-11 of a weight; the output is rounded to bf16, 2^-8) and q, bf16 divided by a power of two, is
 // exact in fp16 down to 2^-16 of the row's largest value.  m is not the running maximum itself but follows it when it is
-// passed by more than 8 (a factor of 256, which fp16 and the fp32 sums take): O in tensor memory is then rescaled, which is rare.
+// passed by more than 8 (a factor of 256, which fp16 and the fp32 sums take): O in tensor memory is then rescaled, which is rare,
+// and so the exponentials need not wait for the maximum of their own step.
 //
-// Bound by the exponentials (16 a clock and SM: 1024 clocks per 128 x 128 tile) and, at head_dim 128, equally by the products.
+// What bounds it: 16 exponentials a clock and SM (1024 clocks for two tiles' step) against 1290 clocks of products at head_dim 128
+// (S at 64 columns is bound by its operands' way through shared memory: 387 clocks where the products alone are 256).  Measured
+// 2500 clocks a step: the three kinds of warps share the schedulers' issue slots.  On the way: one lane in a divergent loop, 128 keys
+// a step and one S buffer 546 us, for 2770 new tokens x 32 heads of 128 behind 2000 to 6000 keys; roles with their own registers 296;
+// two S buffers and 64 keys 281; weights beside their maximum, one body of code (masks go by way of S in tensor memory) 254 us, 800
+// TFLOP/s.  Tried and dropped: two threads per row (349 against 296), polls with a suspend hint (no difference), one tile per
+// block at head_dim 128 (a step of 3100 tokens 89 us against 77).
+// 7.4 thousand prompt tokens of ten heads of 64 take 46 us, half of it the blocks' beginnings and ends (eight steps on average).
 // Where there are few blocks for the GPU the keys are cut into chunks (grid z), whose states the general form's second kernel joins.
 // Every wait is bounded; on expiry the block sets *status, frees its tensor memory and returns.
 #pragma once
@@ -41,8 +50,7 @@ template <int HD, int NT> __host__ __device__ constexpr size_t attn8_tc_smem() {
 }
 
 __device__ __forceinline__ bool wait8(uint32_t bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, kWaitLimitNs); }
-// One lane of a converged warp.  The loop around it stays the same for all lanes, so that addresses and descriptors are kept in
-// uniform registers, where the instruction wants them (a loop run by one lane alone spent about 100 cycles on each).
+// one lane of a converged warp
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(p));
