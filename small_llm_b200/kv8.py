@@ -9,6 +9,14 @@ results and workspace (from torch's allocator, so they can be captured into a CU
     kv8.append(k, v, slot_map, pages, scales)                           # k, v: [n_tok, kv_heads, head_dim]
     out = kv8.attention(q, pages, scales, table, tok_seq, tok_pos, cu_tok, max_new=..., max_len=...)
 
+PagedCache keeps what a decode loop keeps between steps: the layers' pages, the table, the ring of free pages, the lengths.
+
+    cache = kv8.PagedCache(n_layers, n_seqs, n_pages, kv_heads, head_dim, max_len, max_tok)
+    cache.step(len_after)                                               # which sequences grow, shrink or end
+    for layer in ...:
+        cache.append(layer, k, v)                                       # rows of the step's list, cache.tok_seq / tok_pos / cu_tok
+        out = cache.attention(layer, q, max_new=...)
+
 Bad arguments raise ValueError; there is no CPU path.
 """
 from __future__ import annotations
@@ -194,3 +202,57 @@ def attention(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, table:
     else:
         _call(dev, lib.sllm_k_attn_kv8, c, a, None, 0)
     return out
+
+
+class PagedCache:
+    """An 8-bit cache of several layers for up to n_seqs sequences of up to max_len positions (whole pages: rounded up to a multiple
+    of 64), and its bookkeeping on the GPU.
+
+    A step names the length that each sequence is to have after it; from then on lists of up to max_tok new positions say where the
+    rows of k, v and q belong: row t is position tok_pos[t] of sequence tok_seq[t] (-1 behind the last).  Nothing here waits for the GPU,
+    and the buffers stay where they are, so a step with its layers can be captured into a CUDA graph: write the lengths into the
+    tensor that the captured step() was given, and the rows into the captured k, v and q, before each replay.
+
+    A step that needs more pages or entries than there are, or a length above max_len, changes nothing and leaves empty lists:
+    status() says so (0, or the SLLM_ERR_* code), at the cost of a wait for the GPU, and the next step starts from the lengths before."""
+
+    def __init__(self, n_layers: int, n_seqs: int, n_pages: int, kv_heads: int, head_dim: int, max_len: int, max_tok: int, device="cuda"):
+        _need(n_layers > 0 and 0 < n_seqs <= MAX_SEQS and n_pages > 0 and max_len > 0 and max_tok > 0, f"counts must be positive, n_seqs at most {MAX_SEQS}")
+        self.layers = [empty_cache(n_pages, kv_heads, head_dim, device) for _ in range(n_layers)]
+        dev = self.layers[0][0].device
+        i32 = dict(dtype=_I32, device=dev)
+        self.max_len = max_len
+        self.lens = torch.zeros(n_seqs, **i32)
+        self.table = torch.full((n_seqs, (max_len + PAGE - 1) // PAGE), -1, **i32)
+        self.ring = torch.arange(n_pages, **i32)
+        self._pool = torch.tensor([[0, n_pages, 0, 0]] * 2, dtype=_I64, device=dev)
+        self.cu_tok = torch.zeros(n_seqs + 1, **i32)
+        self.tok_seq, self.tok_pos = torch.full((max_tok,), -1, **i32), torch.full((max_tok,), -1, **i32)
+        self.slot_map = torch.full((max_tok,), -1, dtype=_I64, device=dev)
+
+    def step(self, len_after: torch.Tensor) -> None:
+        """Moves every sequence to len_after (int32 [n_seqs] on the cache's device; 0 = it has ended) and makes the step's lists."""
+        now, then = self._pool.unbind(0)
+        block_tables(self.lens, len_after, self.table, self.ring, now, then, self.cu_tok, self.tok_seq, self.tok_pos, self.slot_map)
+        torch.where(then[3] == 0, len_after, self.lens, out=self.lens)
+        now.copy_(then)
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """The step's rows of k and v, [max_tok, kv_heads, head_dim], into a layer."""
+        append(k, v, self.slot_map, *self.layers[layer])
+
+    def attention(self, layer: int, q: torch.Tensor, *, max_new: int = 0, max_len: int = 0, scale: float | None = None, out: torch.Tensor | None = None,
+                  status: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of the step's queries [max_tok, n_heads, head_dim] over a layer.  Rows behind the list's last are left as they
+        are in `out`, and zeros where it is not given."""
+        if out is None:
+            out = torch.zeros_like(q, memory_format=torch.contiguous_format)
+        return attention(q, *self.layers[layer], self.table, self.tok_seq, self.tok_pos, self.cu_tok, max_new=max_new, max_len=max_len or self.max_len, scale=scale,
+                         out=out, status=status)
+
+    def status(self) -> int:
+        """0, or the code of the last step's refusal."""
+        return int(self._pool[1, 3])
+
+    def free_pages(self) -> int:
+        return int(self._pool[0, 1])

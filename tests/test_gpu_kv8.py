@@ -612,6 +612,53 @@ def test_captured_step_replayed_for_other_lengths_and_beside_another():
             s.t.pool[0].copy_(s.t.pool[1])                                   # the captured call reads and writes the same two buffers
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_paged_cache(captured):
+    """Two layers through PagedCache, step by step or as one captured graph: every step's attention is that of fp64 over the rows
+    that the cache stands for, refused steps change nothing, and all pages come back."""
+    L, n, h, grp, d, room = 2, 4, 2, 2, 64, 160
+    cache = kv8.PagedCache(L, n, 14, h, d, max_len=400, max_tok=room)
+    after = torch.zeros(n, dtype=torch.int32, device="cuda")
+    qkv = torch.zeros(L, room, h * grp + 2 * h, d, dtype=torch.bfloat16, device="cuda")
+    outs = [torch.zeros(room, h * grp, d, dtype=torch.bfloat16, device="cuda") for _ in range(L)]
+    split = lambda x: (x[:, :h * grp], x[:, h * grp:h * grp + h], x[:, h * grp + h:])  # noqa: E731
+
+    def step():
+        cache.step(after)
+        for i in range(L):
+            q, k, v = split(qkv[i])
+            cache.append(i, k, v)
+            cache.attention(i, q, out=outs[i])
+
+    graph = None
+    if captured:
+        step()                                                               # lengths are all zero: nothing happens but the loading of kernels
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+    lens = [0] * n
+    for i, (want, code) in enumerate([([100, 1, 0, 30], 0), ([101, 2, 1, 31], 0), ([102, 3, 120, 0], 0), ([102, 3, 281, 1], 4), ([103, 4, 121, 401], 4), ([103, 4, 121, 449], 1),
+                                      ([64, 4, 200, 60], 0),
+                                      ([65, 150, 201, 0], 0), ([400, 150, 201, 0], 4), ([66, 151, 202, 90], 0), ([0, 0, 0, 0], 0)]):
+        after.copy_(torch.tensor(want))
+        qkv.copy_(torch.randn(qkv.shape, device="cuda", generator=gen(i)))
+        graph.replay() if captured else step()
+        assert cache.status() == code
+        lens = want if code == 0 else lens
+        assert cache.lens.tolist() == lens and cache.free_pages() == 14 - sum(ceil(x, PAGE) for x in lens)
+        live = cache.tok_seq >= 0
+        assert code == 0 or not bool(live.any())
+        for j in range(L):
+            q = split(qkv[j])[0]
+            ref, top, smax = plain_attention(q, *cache.layers[j], cache.table, cache.tok_seq, cache.tok_pos, d ** -0.5)
+            err = (outs[j][live].double() - ref[live]).abs()
+            assert bool((err <= _tol(ref, top, smax, 400, d, torch.bfloat16)[live]).all())
+    assert sorted(cache.ring.tolist()) == list(range(14))
+    extra = cache.attention(0, split(qkv[0])[0])
+    assert float(extra.float().abs().max()) == 0.0                           # an empty list
+
+
 # ---- refusals ---------------------------------------------------------------------------------------------------------
 
 def test_refusals():
