@@ -7,13 +7,13 @@
 // integer product, so the products run on the integers themselves: mma.sync with eight query rows (tokens x heads that share
 // a kv head) as its rows 0..7, and what the 8 or 11 bits of an operand leave out of them as its rows 8..15, so that both parts
 // come out in one thread and are added there, at no more matrix instructions than one row costs.  q is first divided by a power
-// of two so that its largest value is in [0.5, 1); p vs is divided by vr, a power of two no smaller than the largest vs so far,
-// which is carried like the running maximum m.  Two forms:
-//   bf16 rows (I8): m16n8k32 on int8, the cache's bytes as they are.  q and p vs / vr become two base-256 digits, 16 bits in
-//     all (2^-16 of the row's largest value: bf16 has 2^-9 of each; 2^-16 of a weight of 1, each key's own, against an output rounded
-//     to 2^-9); products are exact, sums are 32-bit integers.
-//   fp32 rows: m16n8k16 on fp16, in which the integers are exact, q and p vs / vr split into a high and a low fp16 part, 22
-//     bits, fp32 sums: fp32 accuracy.  A byte costs 1.25-1.5 instructions on its way there (xor the sign, byte-permute under 0x64
+// of two so that its largest value is in [0.5, 1); the largest p vs so far is carried beside the running maximum m, so that what the
+// attended values leave room for, and not the loudest value of the cache, sets the precision.  Two forms:
+//   bf16 rows (I8): m16n8k32 on int8, the cache's bytes as they are.  q and p vs become two base-256 digits, 16 bits in all: q
+//     to 2^-16 of the row's largest value (bf16 has 2^-9 of each), p vs to 2^-15 or 2^-16 of the largest p vs there has been (the
+//     output is rounded to 2^-9).  Products are exact, sums are 32-bit integers.
+//   fp32 rows: m16n8k16 on fp16, in which the integers are exact, q and p vs, relative to the same largest, split into a high and
+//     a low fp16 part, 22 bits, fp32 sums: fp32 accuracy.  A byte costs 1.25-1.5 instructions on its way there (xor the sign, byte-permute under 0x64
 //     = 1024 + x, subtract), where I8 spends none on K and half of one on V, to bring four keys of a dim into one register.
 //
 // The kernel is to be bound by HBM: 2 head_dim bytes per cached position and kv head.  A block of threads takes one (row
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     Acc o[VB][4];
 #pragma unroll
     for (int j = 0; j < VB; ++j) { o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0; }
-    float m_run = -INFINITY, l_run = 0.f, vr = 0.f, vr_inv = 0.f;
+    float m_run = -INFINITY, l_run = 0.f, w_run = -INFINITY;
 
     const int n_units = keys > 0 ? (keys + kA8Unit - 1) / kA8Unit : 0;
     const int mine = n_units > warp ? (n_units - warp + kA8Warps - 1) / kA8Warps : 0;
@@ -338,22 +338,26 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
             }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            // The integer form's weights must not pass 1: m moves a little further than it has to, and so less often.
-            const float m_new = mx > m_run ? (I8 ? mx + 1.f : mx) : m_run;
+            const float m_new = fmaxf(m_run, mx);
             const float m_use = m_new == -INFINITY ? 0.f : m_new;
-            float corr = exp2_fast(m_run - m_use);
-            if (I8 && m_run == m_new) corr = 1.f;                // also where both are -inf
+            l_run *= exp2_fast(m_run - m_use);
             m_run = m_new;
-            l_run *= corr;
             // the second block of a unit may lie behind the last position: its scale is another owner's then and does not count
             const float vs0 = scl[4], vs1 = kb + kBlk8 <= last ? scl[5] : 0.f;
-            const float vtop = fmaxf(vs0, vs1);
-            if (vtop > vr) {
-                const float up = pow2_above(fminf(vtop, 1.7e38f));
-                corr *= vr / up;
-                vr = up;
-                vr_inv = 1.f / up;
-            }
+            // The weights of the product with V are p vs relative to the largest there has been, 2^w_run.  Digits must not pass 1, so w_run
+            // moves one further than it has to, and so less often.
+            float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1])) + __log2f(vs0), fmaxf(fmaxf(sc[2][0], sc[2][1]), fmaxf(sc[3][0], sc[3][1])) + __log2f(vs1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float w_new = top > w_run ? top + 1.f : w_run;
+            const float corr = w_new == w_run ? 1.f : exp2_fast(w_run - w_new);          // equal: also where both are -inf
+            w_run = w_new;
+            // p of this step times these
+            const float to_w = w_run == -INFINITY ? 0.f : exp2_fast(fminf(m_use - w_run, 126.f)) * (I8 ? kDigits : 1.f);
+            const float g0 = fminf(vs0 * to_w, 3e38f), g1 = fminf(vs1 * to_w, 3e38f);    // finite: a p of 0 is to stay 0
+            // a scale that is NaN shows by way of the sum: digits carry none, and g does not either
+            if (vs0 != vs0 && kb <= pos) l_run = vs0;
+            if (vs1 != vs1 && kb + kBlk8 <= pos) l_run = vs1;
             if (__any_sync(0xffffffffu, corr != 1.f)) {
 #pragma unroll
                 for (int j = 0; j < VB; ++j)
@@ -363,20 +367,15 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
                         else o[j][k] *= corr;
             }
             if constexpr (I8) {
-                // digits carry no NaN: a scale that is one shows by way of the sum
-                if (vs0 != vs0 && kb <= pos) l_run = vs0;
-                if (vs1 != vs1 && kb + kBlk8 <= pos) l_run = vs1;
                 uint32_t pa[4], x[8];
 #pragma unroll
-                for (int nt = 0; nt < 4; ++nt) {
-                    const float vf = (nt >> 1 ? vs1 : vs0) * vr_inv * kDigits;
+                for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const float p = exp2_fast(sc[nt][e] - m_use);
                         l_run += p;
-                        x[2 * nt + e] = digit_bits(p, vf);
+                        x[2 * nt + e] = digit_bits(p, nt >> 1 ? g1 : g0);
                     }
-                }
                 digits4(x[0], x[1], x[2], x[3], pa[0], pa[1]);
                 digits4(x[4], x[5], x[6], x[7], pa[2], pa[3]);
                 // V: eight keys' rows, (2t, 2t + 1) of each group of 8 as permuted above; four bytes of four rows are turned into four
@@ -407,7 +406,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
             } else {
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
-                const float vf = (kk ? vs1 : vs0) * vr_inv;
+                const float vf = kk ? g1 : g0;
                 uint32_t pa[4];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -469,11 +468,12 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     constexpr int OS = HD + 4;                                   // floats per row: rows start in different banks
     static_assert((size_t)kA8Warps * kA8Rows * OS * 4 <= attn8_smem<HD>(), "the joined states fit the stages");
     float* so = reinterpret_cast<float*>(smem_raw);
+    const float from_w = w_run == -INFINITY ? 0.f : exp2_fast(fminf(w_run - m_run, 126.f)) * (I8 ? 1.f / kDigits : 1.f);      // back to p vs
 #pragma unroll
     for (int j = 0; j < VB; ++j)
 #pragma unroll
         for (int e = 0; e < 2; ++e)                              // column 2t + e of column tile j is dim (2t + e) VB + j
-            so[(warp * kA8Rows + g) * OS + (2 * t + e) * VB + j] = I8 ? fmaf((float)o[j][e], 256.f, (float)o[j][e + 2]) * (vr * (1.f / kDigits)) : (o[j][e] + o[j][e + 2]) * vr;
+            so[(warp * kA8Rows + g) * OS + (2 * t + e) * VB + j] = I8 ? fmaf((float)o[j][e], 256.f, (float)o[j][e + 2]) * from_w : (o[j][e] + o[j][e + 2]) * from_w;
     __syncthreads();
     // eight dims per thread at a time: the four states joined in the order of the warps
     for (int x = tid; x < kA8Rows * HD / 8; x += kA8Threads) {

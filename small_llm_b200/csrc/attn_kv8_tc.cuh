@@ -10,10 +10,11 @@
 //
 // The integers are multiplied as they are (exact in fp16), scales act outside the products and cost nothing per element: with
 // c = scale log2(e) ks(block) and v = vs(block) / vr the weight is  w = p v = exp2(S c + (log2 v - m)),  one fma and one ex2, and
-// the softmax denominator sums w / v block by block.  vr, a power of two no smaller than any vs so far, keeps w in fp16's range.
+// the softmax denominator sums w / v block by block.  vr is a power of two near the first vs, m the largest S c + log2 v so far: what
+// the attended values contribute, and not the loudest value of the cache, is what fp16's range is spent on.
 // w is rounded to fp16 (2^-11 of a weight; the output is rounded to bf16, 2^-8) and q, bf16 divided by a power of two, is
-// exact in fp16 down to 2^-16 of the row's largest value.  m is not the running maximum itself but follows it when it is
-// passed by more than 8 (a factor of 256, which fp16 and the fp32 sums take): O in tensor memory is then rescaled, which is rare,
+// exact in fp16 down to 2^-16 of the row's largest value.  m does not follow every new
+// maximum but one that passes it by more than 8 (a factor of 256, which fp16 and the fp32 sums take): O in tensor memory is then rescaled, which is rare,
 // and so the exponentials need not wait for the maximum of their own step.
 //
 // What bounds it: 16 exponentials a clock and SM (1024 clocks for two tiles' step) against 1290 clocks of products at head_dim 128
@@ -132,7 +133,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
     uint8_t* sQ = smem;                                       // [NT][Q_TILE]
     uint8_t* sK = sQ + NT * Q_TILE;                           // [stages][TILE]
     uint8_t* sV = sK + kT8Stages * TILE;
-    float4* s_blk = reinterpret_cast<float4*>(sV + kT8Stages * TILE);      // [ring][blocks]: c, log2 v, 1 / v, 0 or -inf (blocks that do not count)
+    float4* s_blk = reinterpret_cast<float4*>(sV + kT8Stages * TILE);      // [ring][blocks]: c, log2 v (-inf: does not count), 1 / v
     float4* s_vr = s_blk + kT8Ring * kT8Blks;                 // [ring]: vr
     uint64_t* bars = reinterpret_cast<uint64_t*>(s_vr + kT8Ring);
     // S_READY, P_READY and PV_DONE: [tile][step parity], for they may be a step ahead of who waits
@@ -299,10 +300,12 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
             float top = counts && vs == vs ? vs : 0.f;
 #pragma unroll
             for (int o = 1; o < kT8Blks; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            if (top > vr) vr = pow2_above(fminf(top, 1.7e38f));
+            if (vr == 0.f && top > 0.f) vr = pow2_above(fminf(top, 1.7e38f));
             const float v0 = vr > 0.f ? vs / vr : (vs == 0.f ? 1.f : vs);
-            const float v = v0 != v0 ? v0 : fmaxf(v0, 8.67361738e-19f);              // 2^-60: fp16 takes such a weight for 0, the sum does not
-            const float4 f = counts ? make_float4(ks * fabsf(a.scale) * 1.4426950408889634f, ks == ks ? log2f(v) : ks, 1.f / v, 0.f) : make_float4(0.f, -INFINITY, 0.f, -INFINITY);
+            // Within 2^-60 and 2^100: at the lower end fp16 takes a weight for 0 beside any other, the sum does not; the upper one is
+            // out of reach for values that one model made.
+            const float v = v0 != v0 ? v0 : fminf(fmaxf(v0, 8.67361738e-19f), 1.26765060e30f);
+            const float4 f = counts ? make_float4(ks * fabsf(a.scale) * 1.4426950408889634f, ks == ks ? log2f(v) : ks, 1.f / v, 0.f) : make_float4(0.f, -INFINITY, 0.f, 0.f);
             // the K of a step is free once S is done, which was asked for when the softmax had ended the step two before: with the
             // K of step i - stages free it is done with i - stages - 2, far behind the ring's length
             if (i >= kT8Stages) ok = __all_sync(0xffffffffu, wait8(B(K_FREE + i % kT8Stages), parity(i - kT8Stages)));
@@ -448,7 +451,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
                         top = fmaxf(top, __uint_as_float(x[j]));
                     }
                     if (masked) tc_st16(s_at + b * 16, x);
-                    mx = fmaxf(mx, fmaf(top, fmaxf(blk[b].x * row_f, 1e-37f), blk[b].w));
+                    mx = fmaxf(mx, fmaf(top, fmaxf(blk[b].x * row_f, 1e-37f), blk[b].y));
                 }
                 tc_wait_st();
                 if (i == 0) { m = mx; vr = vr_now; }
@@ -478,7 +481,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
                         t4[0] = fmaxf(fmaxf(t4[0], __uint_as_float(sv[b * 16 + j])), __uint_as_float(sv[b * 16 + j + 1]));
                         if (j + 2 < 16) t4[1] = fmaxf(fmaxf(t4[1], __uint_as_float(sv[b * 16 + j + 2])), __uint_as_float(sv[b * 16 + j + 3]));
                     }
-                    mx = fmaxf(mx, fmaf(fmaxf(t4[0], t4[1]), c, behind ? -INFINITY : f.w));
+                    mx = fmaxf(mx, fmaf(fmaxf(t4[0], t4[1]), c, behind ? -INFINITY : f.y));
                     const unsigned long long c2 = pair2(c, c), d2 = pair2(d, d);
                     unsigned long long sum = 0;
 #pragma unroll

@@ -410,6 +410,26 @@ def test_prompts_with_scales_of_many_magnitudes(d, order):
         check_attention((q.to(rows), pages, scales, table, seq, pos, cu), rows, max_new=1, max_len=300)
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_loud_values_that_nothing_attends(d):
+    """Keys whose weight is next to nothing hold values 2^14 times the others': the result keeps the precision of what is attended."""
+    for dtype, kw in ((torch.bfloat16, dict(max_new=1)), (torch.float32, dict(max_new=1)), (torch.bfloat16, dict(max_new=64, cu_tok=True))):
+        q, pages, scales, table, seq, pos, cu = setup_attention([300, 300], [64, 64], 1, 2, d, dtype, seed=91)
+        sign = torch.sign(q[:1, :1].float())
+        q = (q.float().abs() * sign).to(dtype)                               # all rows point one way
+        row = table[:, 1].long()
+        pages[row, 0, 0] = (-90 * sign[0, 0]).to(torch.int8)                 # keys 64 .. 127 the other way
+        scales[row, 0, 0] = 0.04
+        scales[row, 0, 1] = 0.04 * 2.0 ** 14
+        if kw.get("cu_tok") is not None:
+            kw["cu_tok"] = cu
+        want, _, _ = plain_attention(q, pages, scales, table, seq, pos, d ** -0.5)
+        got = kv8.attention(q, pages, scales, table, seq, pos, max_len=364, **kw).double()
+        assert float(want.abs().max()) < 20                                  # the loud ones are not heard
+        # half a step of bf16 of the value, and 2^-9 of the attended values (at most 127 * 0.04) for the roundings of q, p and vs
+        assert bool(((got - want).abs() <= want.abs() * 2.0 ** -8 + 127 * 0.04 * 2.0 ** -9).all()), (dtype, kw.keys(), float((got - want).abs().max()))
+
+
 def test_prompts_with_bad_pages_and_values_that_are_not_finite():
     q, pages, scales, table, seq, pos, cu = setup_attention([0, 0], [260, 150], 2, 2, 64, torch.bfloat16, seed=78)
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
