@@ -141,7 +141,9 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
            PV_DONE = P_READY + 4, SC_FULL = PV_DONE + 4, Q_FULL = SC_FULL + kT8Ring, N_BARS = Q_FULL + 1 };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
     __shared__ int s_last[2][8];
-    __shared__ int s_len[kT8MaxSort], s_tiles[kT8MaxSort], s_pick[2];
+    __shared__ int2 s_key[kT8MaxSort];                        // last position and tiles of each sequence
+    __shared__ int s_pick[2];
+    __shared__ float s_rowf[NT][kT8Rows];
     const uint32_t bar0 = smem_u32(bars);
     auto B = [&](int i) { return bar0 + 8u * (uint32_t)i; };
 
@@ -156,16 +158,19 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
         for (int i = tid; i < a.n_seq; i += THREADS) {
             const int c0 = a.cu_tok[i], c1 = min(a.cu_tok[i + 1], a.n_tok);
             const bool any = c0 >= 0 && c1 > c0;
-            s_tiles[i] = any ? (c1 - c0 + a.rows_toks - 1) / a.rows_toks : 0;
-            s_len[i] = any ? a.tok_pos[c1 - 1] : -1;
+            s_key[i] = make_int2(any ? a.tok_pos[c1 - 1] : -1, any ? (c1 - c0 + a.rows_toks - 1) / a.rows_toks : 0);
         }
         __syncthreads();
         for (int i = tid; i < a.n_seq; i += THREADS) {
+            const int2 mine = s_key[i];
             int before = 0;
-            const int len = s_len[i];
-            for (int j = 0; j < a.n_seq; ++j) before += s_len[j] > len || (s_len[j] == len && j < i) ? s_tiles[j] : 0;
+#pragma unroll 8
+            for (int j = 0; j < a.n_seq; ++j) {
+                const int2 k = s_key[j];
+                before += (k.x > mine.x) | ((k.x == mine.x) & (j < i)) ? k.y : 0;
+            }
             const int k = (int)blockIdx.y - before;
-            if (k >= 0 && k < s_tiles[i]) { s_pick[0] = i; s_pick[1] = s_tiles[i] - 1 - k; }
+            if (k >= 0 && k < mine.y) { s_pick[0] = i; s_pick[1] = mine.y - 1 - k; }
         }
         __syncthreads();
         seq = s_pick[0];
@@ -179,23 +184,6 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
     const int head = blockIdx.x, group = a.group, toks = a.rows_toks / NT;   // tokens of one tile
     const int most = (int)min((long long)a.width * kPage, 0x7fffff00ll) - 1;
 
-    // last position of each tile's tokens
-    if (tid < 2 * kT8Rows) {
-        const int pos = tid < n ? min(a.tok_pos[t0 + tid], most) : -1;
-        const int p0 = __reduce_max_sync(0xffffffffu, tid < toks ? pos : -1), p1 = __reduce_max_sync(0xffffffffu, tid < toks ? -1 : pos);
-        if (lane == 0) { s_last[0][warp] = p0; s_last[1][warp] = p1; }
-    }
-    __syncthreads();
-    int last0 = -1, last1 = -1;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { last0 = max(last0, s_last[0][i]); last1 = max(last1, s_last[1][i]); }
-    // This block's chunk of the keys: from here on positions and pages count from its first key.  The last chunk takes all that is left.
-    const int chunk = blockIdx.z, key0 = chunk * a.chunk, own_chunks = attn8_chunks(a, max(last0, last1));
-    const int last = max(last0, last1) - key0, most_steps = chunk == a.n_chunks - 1 ? 0x7fffffff : a.chunk / kT8Keys;
-    const int n0 = min(max(last0 - key0 + kT8Keys, 0) / kT8Keys, most_steps), n1 = min(max(last1 - key0 + kT8Keys, 0) / kT8Keys, most_steps);
-    const int steps = max(n0, n1);                            // 0 where nothing is attended
-    if (steps == 0 && chunk > 0) return;                      // chunk 0 writes the rows that attend nothing
-
     if (tid == 0) {
         for (int i = 0; i < kT8Stages; ++i) { mbar_init(B(K_FULL + i), 5); mbar_init(B(V_FULL + i), 4); mbar_init(B(K_FREE + i), 1); mbar_init(B(V_FREE + i), 1); }
         for (int i = 0; i < 4; ++i) { mbar_init(B(S_READY + i), 1); mbar_init(B(P_READY + i), 4); mbar_init(B(PV_DONE + i), 1); }
@@ -207,11 +195,29 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-
+    // last position of each tile's tokens
+    if (tid < 2 * kT8Rows) {
+        const int pos = tid < n ? min(a.tok_pos[t0 + tid], most) : -1;
+        const int p0 = __reduce_max_sync(0xffffffffu, tid < toks ? pos : -1), p1 = __reduce_max_sync(0xffffffffu, tid < toks ? -1 : pos);
+        if (lane == 0) { s_last[0][warp] = p0; s_last[1][warp] = p1; }
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    int last0 = -1, last1 = -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { last0 = max(last0, s_last[0][i]); last1 = max(last1, s_last[1][i]); }
+    // This block's chunk of the keys: from here on positions and pages count from its first key.  The last chunk takes all that is left.
+    const int chunk = blockIdx.z, key0 = chunk * a.chunk, own_chunks = attn8_chunks(a, max(last0, last1));
+    const int last = max(last0, last1) - key0, most_steps = chunk == a.n_chunks - 1 ? 0x7fffffff : a.chunk / kT8Keys;
+    const int n0 = min(max(last0 - key0 + kT8Keys, 0) / kT8Keys, most_steps), n1 = min(max(last1 - key0 + kT8Keys, 0) / kT8Keys, most_steps);
+    const int steps = max(n0, n1);                            // 0 where nothing is attended
+    if (steps == 0 && chunk > 0) {                            // chunk 0 writes the rows that attend nothing
+        if (warp == SOFT + WIDE) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
+        return;
+    }
+
     bool ok = true;
 
     const int* table = a.table + (size_t)seq * a.width + key0 / kPage;
@@ -378,51 +384,58 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
     } else {
         // ---- softmax: thread = query row = TMEM lane ----
         if constexpr (NT == 2) more_registers<144>(); else more_registers<136>();
-        // this thread's row: q as fp16, K-major with the 128-byte swizzle; rows of no token are zero
+        // This thread's row; and the warp's 32 rows of q as fp16, K-major with the 128-byte swizzle, read and written by HD / 8 lanes each.
+        // Rows of no token are zero.
         const int tile = warp >> 2, r = tid & 127;
         int pos = 0, row_tok = -1, row_head = 0;
-        float row_f = 0.f;
+        if (r / group < toks && tile * toks + r / group < n) { row_tok = t0 + tile * toks + r / group; row_head = head * group + r % group; }
+        pos = row_tok >= 0 ? min(a.tok_pos[row_tok], most) - key0 : -1;
         {
-            const int rt = tile * toks + r / group;
-            const bool valid = r / group < toks && rt < n;
-            if (valid) { row_tok = t0 + rt; row_head = head * group + r % group; }
-            pos = valid ? min(a.tok_pos[row_tok], most) - key0 : -1;
-            uint4 raw[HD / 8];
-            const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + (valid ? (long long)row_tok * a.q_stride + row_head * HD : 0);
-            unsigned top = 0;
+            constexpr int CH = HD / 8, RPI = 32 / CH;          // lanes per row, rows at a time
+            const int c = lane % CH;
+#pragma unroll 1
+            for (int b = 0; b < CH; b += 8) {
+                uint4 raw[8];
 #pragma unroll
-            for (int c = 0; c < HD / 8; ++c) {
-                raw[c] = make_uint4(0u, 0u, 0u, 0u);
-                if (valid) {
-                    if (a.wide) raw[c] = *reinterpret_cast<const uint4*>(src + 8 * c);
-                    else {
-                        uint32_t w[4];
+                for (int i = 0; i < 8; ++i) {
+                    const int rr = (r & ~31) + (b + i) * RPI + lane / CH, rt = tile * toks + rr / group;
+                    raw[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (rr / group < toks && rt < n) {
+                        const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + (long long)(t0 + rt) * a.q_stride + (head * group + rr % group) * HD + c * 8;
+                        if (a.wide) raw[i] = *reinterpret_cast<const uint4*>(src);
+                        else {
+                            uint32_t w[4];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            w[j] = (uint32_t)__bfloat16_as_ushort(src[8 * c + 2 * j]) | (uint32_t)__bfloat16_as_ushort(src[8 * c + 2 * j + 1]) << 16;
-                        raw[c] = make_uint4(w[0], w[1], w[2], w[3]);
+                            for (int j = 0; j < 4; ++j) w[j] = (uint32_t)__bfloat16_as_ushort(src[2 * j]) | (uint32_t)__bfloat16_as_ushort(src[2 * j + 1]) << 16;
+                            raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
                     }
                 }
-                const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[c]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) top = max(top, max((w[j] & 0x7fffu) << 16, w[j] & 0x7fff0000u));
-            }
-            // f = 2^-e with the largest value in [2^(e-1), 2^e), as in the general kernel
-            const int e = min(max((int)(top >> 23) - 126, -125), 125);
-            const float f = top ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
-            row_f = top ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
-            const float fs = a.scale < 0.f ? -f : f;              // block factors are positive: a maximum may be taken before them
+                for (int i = 0; i < 8; ++i) {
+                    const int rr = (r & ~31) + (b + i) * RPI + lane / CH;
+                    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
+                    unsigned top = 0;
 #pragma unroll
-            for (int c = 0; c < HD / 8; ++c) {
-                float x[8];
-                unpack16<__nv_bfloat16>(raw[c], x);
-                *reinterpret_cast<uint4*>(sQ + tile * Q_TILE + (c >> 3) * Q_HALF + sw128(r, c & 7)) =
-                    make_uint4(pack_half(x[0] * fs, x[1] * fs), pack_half(x[2] * fs, x[3] * fs), pack_half(x[4] * fs, x[5] * fs), pack_half(x[6] * fs, x[7] * fs));
+                    for (int j = 0; j < 4; ++j) top = max(top, max((w[j] & 0x7fffu) << 16, w[j] & 0x7fff0000u));
+#pragma unroll
+                    for (int o = 1; o < CH; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    // f = 2^-e with the largest value in [2^(e-1), 2^e), as in the general form
+                    const int e = min(max((int)(top >> 23) - 126, -125), 125);
+                    const float f = top ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
+                    if (c == 0) s_rowf[tile][rr] = top ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
+                    const float fs = a.scale < 0.f ? -f : f;   // block factors are positive: a maximum may be taken before them
+                    float x[8];
+                    unpack16<__nv_bfloat16>(raw[i], x);
+                    *reinterpret_cast<uint4*>(sQ + tile * Q_TILE + (c >> 3) * Q_HALF + sw128(rr, c & 7)) =
+                        make_uint4(pack_half(x[0] * fs, x[1] * fs), pack_half(x[2] * fs, x[3] * fs), pack_half(x[4] * fs, x[5] * fs), pack_half(x[6] * fs, x[7] * fs));
+                }
             }
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(B(Q_FULL));
         }
+        const float row_f = s_rowf[tile][r];
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t o_at = lanes + NT * 2 * kT8Keys + tile * HD;
         const int my_steps = tile ? n1 : n0;
