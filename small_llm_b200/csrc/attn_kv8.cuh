@@ -111,9 +111,9 @@ __device__ __forceinline__ float pow2_above(float x) {
     const uint32_t u = __float_as_uint(x);
     return __uint_as_float((u + 0x007fffffu) & 0x7f800000u);
 }
-// the row tile of a block: tokens [t0, t0 + n) of one sequence (n = 0: nothing to do)
-__device__ __forceinline__ int attn8_tile(const Attn8Args& a, int tile, int& t0, int& seq) {
-    if (!a.cu_tok) {
+// the row tile of a block: tokens [t0, t0 + n) of one sequence (n = 0: nothing to do); cu: a.cu_tok, or a copy of it
+__device__ __forceinline__ int attn8_tile(const Attn8Args& a, const int* cu, int tile, int& t0, int& seq) {
+    if (!cu) {
         t0 = tile;
         seq = a.tok_seq[tile];
         return seq >= 0 && seq < a.n_seq ? 1 : 0;
@@ -122,15 +122,14 @@ __device__ __forceinline__ int attn8_tile(const Attn8Args& a, int tile, int& t0,
     int lo = 0, hi = a.n_seq;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (a.cu_tok[mid] / a.rows_toks + mid <= tile) lo = mid; else hi = mid;
+        if (cu[mid] / a.rows_toks + mid <= tile) lo = mid; else hi = mid;
     }
-    const int first = a.cu_tok[lo];
-    const int end = min(a.cu_tok[lo + 1], a.n_tok);
+    const int first = cu[lo];
+    const int end = min(cu[lo + 1], a.n_tok);
     t0 = first + (tile - first / a.rows_toks - lo) * a.rows_toks;
     seq = lo;
     return first >= 0 && t0 >= 0 ? min(a.rows_toks, end - t0) : 0;
 }
-
 constexpr int kA8MaxCluster = 8;       // blocks of a cluster: what every GPU grants
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -184,7 +183,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     // heads follow on one another: the blocks that run side by side read the same pages, whose heads lie next to each other
     const int per_tile = a.c.H * a.head_tiles, tile = blockIdx.x / per_tile, in_tile = blockIdx.x % per_tile;
     int t0, seq;
-    const int n = attn8_tile(a, tile, t0, seq);
+    const int n = attn8_tile(a, a.cu_tok, tile, t0, seq);
     if (n <= 0) return;
     const int head = in_tile / a.head_tiles, ht = in_tile % a.head_tiles;
     const int chunk = blockIdx.z;

@@ -39,7 +39,8 @@ constexpr int kT8Blks = kT8Keys / kBlk8;         // scale blocks of a step
 constexpr int kT8Ring = 8;                       // steps whose scales are held
 constexpr int kT8Stages = 4;                     // widened K (and V) tiles
 constexpr float kT8Slack = 8.f;                  // log2 units that scores may pass m by
-constexpr int kT8MaxSort = 256;                  // sequences up to which blocks order the tiles by their keys
+constexpr int kT8MaxSort = 64;                   // sequences up to which blocks order the tiles by their keys
+constexpr int kT8MaxCu = 1024;                   // sequences up to which a tile is looked for in shared memory
 
 // NT tiles of query rows per block.  Warps: 4 NT softmax; 4 widening K and 4 widening V (NT = 1: 4 for both); the last four are
 // the MMA warp, the scales' warp and two that idle.  Registers are dealt out again at the start (setmaxnreg): the launch has
@@ -142,6 +143,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
     __shared__ int s_last[2][8];
     __shared__ int2 s_key[kT8MaxSort];                        // last position and tiles of each sequence
+    __shared__ int s_cu[kT8MaxCu + 1];
     __shared__ int s_pick[2];
     __shared__ float s_rowf[NT][kT8Rows];
     const uint32_t bar0 = smem_u32(bars);
@@ -179,7 +181,14 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
             t0 = c0 + s_pick[1] * a.rows_toks;
             n = min(a.rows_toks, min(a.cu_tok[seq + 1], a.n_tok) - t0);
         }
-    } else n = attn8_tile(a, gridDim.y - 1 - blockIdx.y, t0, seq);
+    } else {
+        const bool fits = a.n_seq <= kT8MaxCu;
+        if (fits) {
+            for (int i = tid; i <= a.n_seq; i += THREADS) s_cu[i] = a.cu_tok[i];
+            __syncthreads();
+        }
+        n = attn8_tile(a, fits ? s_cu : a.cu_tok, gridDim.y - 1 - blockIdx.y, t0, seq);
+    }
     if (n <= 0) return;
     const int head = blockIdx.x, group = a.group, toks = a.rows_toks / NT;   // tokens of one tile
     const int most = (int)min((long long)a.width * kPage, 0x7fffff00ll) - 1;
@@ -393,15 +402,16 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
         {
             constexpr int CH = HD / 8, RPI = 32 / CH;          // lanes per row, rows at a time
             const int c = lane % CH;
+            const unsigned per = (65536u + group - 1) / group;  // rr / group = rr * per >> 16 for rr < 128
 #pragma unroll 1
             for (int b = 0; b < CH; b += 8) {
                 uint4 raw[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const int rr = (r & ~31) + (b + i) * RPI + lane / CH, rt = tile * toks + rr / group;
+                    const int rr = (r & ~31) + (b + i) * RPI + lane / CH, in = (int)((rr * per) >> 16), rt = tile * toks + in;
                     raw[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (rr / group < toks && rt < n) {
-                        const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + (long long)(t0 + rt) * a.q_stride + (head * group + rr % group) * HD + c * 8;
+                    if (in < toks && rt < n) {
+                        const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + (long long)(t0 + rt) * a.q_stride + (head * group + rr - in * group) * HD + c * 8;
                         if (a.wide) raw[i] = *reinterpret_cast<const uint4*>(src);
                         else {
                             uint32_t w[4];
