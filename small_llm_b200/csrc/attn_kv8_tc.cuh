@@ -421,24 +421,36 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
                         }
                     }
                 }
+                // rows whose maxima go through the shuffles side by side (all eight at head_dim 128: the registers that this takes from the steps
+                // cost 5 %)
+                constexpr int SIDE = HD == 64 ? 8 : 1;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int rr = (r & ~31) + (b + i) * RPI + lane / CH;
-                    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
-                    unsigned top = 0;
+                for (int i0 = 0; i0 < 8; i0 += SIDE) {
+                    unsigned top[SIDE];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) top = max(top, max((w[j] & 0x7fffu) << 16, w[j] & 0x7fff0000u));
+                    for (int i = 0; i < SIDE; ++i) {
+                        const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i0 + i]);
+                        top[i] = 0;
 #pragma unroll
-                    for (int o = 1; o < CH; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    // f = 2^-e with the largest value in [2^(e-1), 2^e), as in the general form
-                    const int e = min(max((int)(top >> 23) - 126, -125), 125);
-                    const float f = top ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
-                    if (c == 0) s_rowf[tile][rr] = top ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
-                    const float fs = a.scale < 0.f ? -f : f;   // block factors are positive: a maximum may be taken before them
-                    float x[8];
-                    unpack16<__nv_bfloat16>(raw[i], x);
-                    *reinterpret_cast<uint4*>(sQ + tile * Q_TILE + (c >> 3) * Q_HALF + sw128(rr, c & 7)) =
-                        make_uint4(pack_half(x[0] * fs, x[1] * fs), pack_half(x[2] * fs, x[3] * fs), pack_half(x[4] * fs, x[5] * fs), pack_half(x[6] * fs, x[7] * fs));
+                        for (int j = 0; j < 4; ++j) top[i] = max(top[i], max((w[j] & 0x7fffu) << 16, w[j] & 0x7fff0000u));
+                    }
+#pragma unroll
+                    for (int o = 1; o < CH; o <<= 1)
+#pragma unroll
+                        for (int i = 0; i < SIDE; ++i) top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+#pragma unroll
+                    for (int i = 0; i < SIDE; ++i) {
+                        const int rr = (r & ~31) + (b + i0 + i) * RPI + lane / CH;
+                        // f = 2^-e with the largest value in [2^(e-1), 2^e), as in the general form
+                        const int e = min(max((int)(top[i] >> 23) - 126, -125), 125);
+                        const float f = top[i] ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
+                        if (c == 0) s_rowf[tile][rr] = top[i] ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
+                        const float fs = a.scale < 0.f ? -f : f;   // block factors are positive: a maximum may be taken before them
+                        float x[8];
+                        unpack16<__nv_bfloat16>(raw[i0 + i], x);
+                        *reinterpret_cast<uint4*>(sQ + tile * Q_TILE + (c >> 3) * Q_HALF + sw128(rr, c & 7)) =
+                            make_uint4(pack_half(x[0] * fs, x[1] * fs), pack_half(x[2] * fs, x[3] * fs), pack_half(x[4] * fs, x[5] * fs), pack_half(x[6] * fs, x[7] * fs));
+                    }
                 }
             }
             fence_async_smem();
