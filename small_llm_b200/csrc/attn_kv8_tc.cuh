@@ -43,12 +43,12 @@ constexpr int kT8MaxSort = 64;                   // sequences up to which blocks
 constexpr int kT8MaxCu = 1024;                   // sequences up to which a tile is looked for in shared memory
 
 // NT tiles of query rows per block.  Warps: 4 NT softmax; 4 widening K and 4 widening V (NT = 1: 4 for both); the last four are
-// the MMA warp, the scales' warp and two that idle.  Registers are dealt out again at the start (setmaxnreg): the launch has
-// 640 x 96 = 61440 (NT = 1: 384 x 80 = 30720 per block, two blocks), of which the softmax takes 256 x 144 (128 x 136), the
-// widening 256 x 72 (128 x 64) and the last four warps 128 x 48 (128 x 40): 61440 (30720).
+// the MMA warp, the scales' warp and two that idle.  Registers are dealt out again at the start (setmaxnreg).  In units of 128 threads, NT = 2:
+// launched with 5 x 96 = 480; softmax 2 x 144, widening 2 x 72, the last four warps 48: 480.  NT = 1: 3 x 80 = 240; 136, 64, 40: 240.
 template <int NT> __host__ __device__ constexpr int attn8_tc_threads() { return NT == 2 ? 640 : 384; }
+constexpr int kT8BarBytes = 512;                 // barriers, and where the tensor memory begins
 template <int HD, int NT> __host__ __device__ constexpr size_t attn8_tc_smem() {
-    return 1024 + NT * (size_t)kT8Rows * HD * 2 + 2 * kT8Stages * (size_t)kT8Keys * HD * 2 + kT8Ring * (kT8Blks + 1) * 16 + 256;
+    return 1024 + NT * (size_t)kT8Rows * HD * 2 + 2 * kT8Stages * (size_t)kT8Keys * HD * 2 + kT8Ring * (kT8Blks + 1) * 16 + kT8BarBytes;
 }
 
 __device__ __forceinline__ bool wait8(uint32_t bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, kWaitLimitNs); }
@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
     // S_READY, P_READY and PV_DONE: [tile][step parity], for they may be a step ahead of who waits
     enum { K_FULL = 0, V_FULL = K_FULL + kT8Stages, K_FREE = V_FULL + kT8Stages, V_FREE = K_FREE + kT8Stages, S_READY = V_FREE + kT8Stages, P_READY = S_READY + 4,
            PV_DONE = P_READY + 4, SC_FULL = PV_DONE + 4, Q_FULL = SC_FULL + kT8Ring, N_BARS = Q_FULL + 1 };
+    static_assert(N_BARS * 8 + 4 <= kT8BarBytes, "the barriers fit their place");
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
     __shared__ int s_last[2][8];
     __shared__ int2 s_key[kT8MaxSort];                        // last position and tiles of each sequence

@@ -29,8 +29,7 @@ int bad(const char* what, const char* why) {
     return fail_text(SLLM_ERR_INVALID, b);
 }
 
-// What the checks and the launch rules need to know of a device, looked up once.
-struct Device { int sms = 0; };
+// The current device and its SM count, which is looked up once.
 int current_device(const char* what, int* dev, int* sms) {
     static std::atomic<int> known[kMaxDev];          // SM count, 0 = not looked up
     if (cudaError_t err = cudaGetDevice(dev)) { (void)cudaGetLastError(); return cuda_fail(err, what); }

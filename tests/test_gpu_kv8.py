@@ -379,6 +379,16 @@ def test_long_prompts(h, grp, d):
     check_attention(b, torch.bfloat16, max_new=90, max_len=3090, cu_tok=b[6], scale=-0.2)
 
 
+@pytest.mark.parametrize("n,grp,d", [(64, 16, 64), (65, 16, 128), (300, 32, 64), (1100, 64, 64)])
+def test_prompts_of_many_sequences(n, grp, d):
+    """Each way in which a block finds its tile: sorted, in a copy of the offsets, in the offsets themselves; empty sequences among them."""
+    r = np.random.RandomState(n)
+    new = [int(x) for x in r.choice([0, 1, 3, 5, 9] if n < 500 else [0, 0, 1, 2], n)]
+    a = setup_attention([int(x) for x in r.randint(0, 200, n)], new, 1, grp, d, torch.bfloat16, seed=n)
+    assert sum(new) * grp >= 40 * n                                          # enough rows for the tensor-core form
+    check_attention(a, torch.bfloat16, max_new=9, max_len=210, cu_tok=a[6])
+
+
 @pytest.mark.parametrize("h,grp,d", [(1, 1, 64), (2, 4, 128), (1, 3, 64)])
 def test_prompts_behind_long_histories_in_chunks(h, grp, d):
     """Few query rows and many keys: the keys of a tile in chunks, of which short sequences have one and some rows attend none."""
