@@ -21,10 +21,10 @@
 // (S at 64 columns is bound by its operands' way through shared memory: 387 clocks where the products alone are 256).  Measured
 // 2500 clocks a step: the three kinds of warps share the schedulers' issue slots.  On the way: one lane in a divergent loop, 128 keys
 // a step and one S buffer 546 us, for 2770 new tokens x 32 heads of 128 behind 2000 to 6000 keys; roles with their own registers 296;
-// two S buffers and 64 keys 281; weights beside their maximum, one body of code (masks go by way of S in tensor memory) 254 us, 800
-// TFLOP/s.  Tried and dropped: two threads per row (349 against 296), polls with a suspend hint (no difference), one tile per
-// block at head_dim 128 (a step of 3100 tokens 89 us against 77).
-// 7.4 thousand prompt tokens of ten heads of 64 take 46 us, half of it the blocks' beginnings and ends (eight steps on average).
+// two S buffers and 64 keys 281; weights beside their maximum, one body of code (masks go by way of S in tensor memory) 254; query rows read
+// by lanes side by side 240 us, 850 TFLOP/s.  Tried and dropped: two threads per row (349 against 296), polls with a suspend hint (no difference), one tile per
+// block at head_dim 128 (a step of 3100 tokens 89 us against 77 then).
+// 7.4 thousand prompt tokens of ten heads of 64 take 44 us, half of it the blocks' beginnings and ends (eight steps on average).
 // Where there are few blocks for the GPU the keys are cut into chunks (grid z), whose states the general form's second kernel joins.
 // Every wait is bounded; on expiry the block sets *status, frees its tensor memory and returns.
 #pragma once
