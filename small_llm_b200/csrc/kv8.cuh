@@ -232,12 +232,12 @@ constexpr int kAppendWindow = 16;      // list entries whose leaders one block h
 // it, and goes when the block is started anew.  The smallest scale of a block with anything in it is 2^-126, so that 1 / s
 // is finite.
 // A block of threads takes the leaders among 16 list entries (31 slots say where their runs end).  The rows are read once and
-// kept in registers between the maximum and the rounding; at head_dim 128 two warps share a block of 16 rows, so that four
-// blocks of threads and not two fit an SM.  Bound by the bytes of long lists and the round trips to them, by latency in short ones:
-// 2.5 us for 64 rows of ten heads of 64, 17.5 us for 7.4 thousand (28 MB), 20 us for eight thousand fp32 rows of eight heads of 128 (82 MB,
+// kept in registers between the maximum and the rounding; at head_dim 128 two warps share a block of 16 rows, and registers are
+// held to 80, so that three blocks of threads and not two fit an SM.  Bound by the bytes of long lists and the round trips to them, by latency in short ones:
+// 2.5 us for 64 rows of ten heads of 64, 14.6 us for 7.4 thousand (28 MB; 17.5 with two blocks per SM), 20 us for eight thousand fp32 rows of eight heads of 128 (82 MB,
 // 4.1 TB/s; 42 us with one warp per block and conversion instructions).
 template <typename T, int HD>
-__global__ void __launch_bounds__(kAppendWarps * 32) k_kv8_append(const Append8Args a) {
+__global__ void __launch_bounds__(kAppendWarps * 32, 3) k_kv8_append(const Append8Args a) {
     constexpr int VPR = HD / 8;                         // vectors of 8 per row
     constexpr int W = HD / 128 + 1, TEAM = W * 32;      // warps, threads of a unit
     constexpr int VPL = (kBlk8 * VPR + TEAM - 1) / TEAM;        // vectors per thread and unit
