@@ -351,9 +351,9 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
             const float w_new = top > w_run ? top + 1.f : w_run;
             const float corr = w_new == w_run ? 1.f : exp2_fast(w_run - w_new);          // equal: also where both are -inf
             w_run = w_new;
-            // p of this step times these
-            const float to_w = w_run == -INFINITY ? 0.f : exp2_fast(fminf(m_use - w_run, 126.f)) * (I8 ? kDigits : 1.f);
-            const float g0 = fminf(vs0 * to_w, 3e38f), g1 = fminf(vs1 * to_w, 3e38f);    // finite: a p of 0 is to stay 0
+            // p of this step times these.  2^(m - w_run) in two halves: neither overflows beside a vs that is as far from 1.
+            const float half_w = w_run == -INFINITY ? 0.f : exp2_fast(fminf(fmaxf(0.5f * (m_use - w_run), -126.f), 126.f));
+            const float k = I8 ? kDigits : 1.f, g0 = fminf(vs0 * half_w * k * half_w, 3e38f), g1 = fminf(vs1 * half_w * k * half_w, 3e38f);     // finite: a p of 0 stays 0
             // a scale that is NaN shows by way of the sum: digits carry none, and g does not either
             if (vs0 != vs0 && kb <= pos) l_run = vs0;
             if (vs1 != vs1 && kb + kBlk8 <= pos) l_run = vs1;
@@ -467,12 +467,12 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     constexpr int OS = HD + 4;                                   // floats per row: rows start in different banks
     static_assert((size_t)kA8Warps * kA8Rows * OS * 4 <= attn8_smem<HD>(), "the joined states fit the stages");
     float* so = reinterpret_cast<float*>(smem_raw);
-    const float from_w = w_run == -INFINITY ? 0.f : exp2_fast(fminf(w_run - m_run, 126.f)) * (I8 ? 1.f / kDigits : 1.f);      // back to p vs
+    const float from_w = w_run == -INFINITY ? 0.f : exp2_fast(fminf(fmaxf(0.5f * (w_run - m_run), -126.f), 126.f));      // back to p vs, by halves as well
 #pragma unroll
     for (int j = 0; j < VB; ++j)
 #pragma unroll
         for (int e = 0; e < 2; ++e)                              // column 2t + e of column tile j is dim (2t + e) VB + j
-            so[(warp * kA8Rows + g) * OS + (2 * t + e) * VB + j] = I8 ? fmaf((float)o[j][e], 256.f, (float)o[j][e + 2]) * from_w : (o[j][e] + o[j][e + 2]) * from_w;
+            so[(warp * kA8Rows + g) * OS + (2 * t + e) * VB + j] = (I8 ? fmaf((float)o[j][e], 256.f, (float)o[j][e + 2]) * (1.f / kDigits) : (float)o[j][e] + (float)o[j][e + 2]) * from_w * from_w;
     __syncthreads();
     // eight dims per thread at a time: the four states joined in the order of the warps
     for (int x = tid; x < kA8Rows * HD / 8; x += kA8Threads) {

@@ -483,6 +483,22 @@ def test_peaked_and_extreme_scores():
         check_attention((q,) + a[1:], torch.float32, max_new=1, max_len=701, scale=1.0 / m)
 
 
+@pytest.mark.parametrize("d", [16, 64, 128])
+def test_values_of_extreme_magnitude(d):
+    """V scaled by a power of two scales the result by it, whatever the form; a block of zeros among them."""
+    for dtype, kw in ((torch.float32, dict(max_new=1)), (torch.bfloat16, dict(max_new=1)), (torch.bfloat16, dict())):
+        q, pages, scales, table, seq, pos, cu = setup_attention([300, 40], [60, 60], 1, 2, d, dtype, seed=23)
+        scales[int(table[0, 1]), 0, 1, 2] = 0.0
+        kw = dict(kw, max_len=360, **({} if kw else dict(cu_tok=cu)))
+        base = kv8.attention(q, pages, scales, table, seq, pos, **kw).double()
+        for e in (-104, -60, 60, 104):
+            loud = scales.clone()
+            loud[:, :, 1] *= 2.0 ** e
+            got = kv8.attention(q, pages, loud, table, seq, pos, **kw).double() * 2.0 ** -e
+            top = base.abs().amax(-1, keepdim=True)
+            assert bool(((got - base).abs() <= top * (2.0 ** -6 if dtype == torch.bfloat16 else 2.0 ** -18)).all()), (dtype, e)
+
+
 def test_values_that_are_not_finite():
     """A NaN scale shows in the rows that attend its block and in no other; a NaN query in its own row."""
     a = setup_attention([100, 100, 15], [1, 1, 1], 2, 2, 64, torch.float32, seed=8)
