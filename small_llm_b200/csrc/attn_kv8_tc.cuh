@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
         if (steps > 0) fetch(0);
         for (int i = 0; i < steps && ok; ++i) {
             id = lane < kT8Blks && i + 1 < steps ? page_of(i + 1) : -1;
-            float top = counts && vs == vs ? vs : 0.f;
+            float top = counts && vs < INFINITY ? vs : 0.f;          // one that is not finite is no reference
 #pragma unroll
             for (int o = 1; o < kT8Blks; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             if (vr == 0.f && top > 0.f) vr = pow2_above(fminf(top, 1.7e38f));
@@ -508,9 +508,9 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
                 for (int b = 0; b < 4; ++b) {
                     const float4 f = blk[b];
                     // c stays above zero so that -inf stays -inf (a block's factor that is NaN comes by f.y); a block behind the row
-                    // does not count, whatever it holds
+                    // does not count, whatever it holds: its factors, which may be infinite or NaN, are not used in the maximum, the weights or the sum
                     const bool behind = k0 + b * 16 > open;
-                    const float c = fmaxf(f.x * row_f, 1e-37f), d = behind ? -INFINITY : f.y - m_use;
+                    const float c = behind ? 1e-37f : fmaxf(f.x * row_f, 1e-37f), d = behind ? -INFINITY : f.y - m_use;
                     float t4[2] = {__uint_as_float(sv[b * 16]), __uint_as_float(sv[b * 16 + 1])};
 #pragma unroll
                     for (int j = 2; j < 16; j += 4) {
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
                         pk[b * 8 + j / 2] = pack_half(w0, w1);
                     }
                     const float2 s2 = unpair2(sum);
-                    l_add = fmaf(s2.x + s2.y, f.z, l_add);
+                    l_add = fmaf(s2.x + s2.y, behind ? 0.f : f.z, l_add);
                 }
                 const bool moves = mx > m + kT8Slack || (m == -INFINITY && mx > m);
                 if (!__any_sync(0xffffffffu, moves || vr_now != vr)) break;
