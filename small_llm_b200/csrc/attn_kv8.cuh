@@ -190,8 +190,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     // this lane's row
     const int r_tok = g / a.rows_heads, r_head = ht * a.rows_heads + g % a.rows_heads;
     const bool row_ok = r_tok < n && r_head < a.group;
-    const long long most = (long long)a.width * kPage - 1;
-    const int pos = row_ok ? (int)min((long long)a.tok_pos[t0 + r_tok], most) : -1;
+    const int pos = row_ok ? max(min(a.tok_pos[t0 + r_tok], a.width * kPage - 1), -1) : -1;      // width * 64 is at most 2^30; not below -1: no difference wraps
     int last = pos;
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));

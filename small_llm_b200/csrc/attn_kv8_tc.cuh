@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
     }
     // last position of each tile's tokens
     if (tid < 2 * kT8Rows) {
-        const int pos = tid < n ? min(a.tok_pos[t0 + tid], most) : -1;
+        const int pos = tid < n ? max(min(a.tok_pos[t0 + tid], most), -1) : -1;
         const int p0 = __reduce_max_sync(0xffffffffu, tid < toks ? pos : -1), p1 = __reduce_max_sync(0xffffffffu, tid < toks ? -1 : pos);
         if (lane == 0) { s_last[0][warp] = p0; s_last[1][warp] = p1; }
     }
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
         const int tile = warp >> 2, r = tid & 127;
         int pos = 0, row_tok = -1, row_head = 0;
         if (r / group < toks && tile * toks + r / group < n) { row_tok = t0 + tile * toks + r / group; row_head = head * group + r % group; }
-        pos = row_tok >= 0 ? min(a.tok_pos[row_tok], most) - key0 : -1;
+        pos = row_tok >= 0 ? max(min(a.tok_pos[row_tok], most), -1) - key0 : -1;      // tok_pos may be anything: a difference must not wrap
         {
             constexpr int CH = HD / 8, RPI = 32 / CH;          // lanes per row, rows at a time
             const int c = lane % CH;

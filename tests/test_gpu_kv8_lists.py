@@ -1,0 +1,32 @@
+"""Lists that say nothing to do, or that contradict one another, in every form of the 8-bit cache's attention: rows alone, rows
+of a cluster's chunks, chunks by way of the workspace, the prompt form whole and in chunks."""
+import pytest
+import torch
+
+from small_llm_b200 import kv8
+
+from .test_gpu_kv8 import TYPES, check_attention, setup_attention
+
+pytestmark = pytest.mark.gpu
+LOWEST = -2 ** 31
+
+
+@pytest.mark.parametrize("far", [-2, LOWEST, LOWEST + 1, LOWEST + 5000])
+@pytest.mark.parametrize("h,grp,d", [(1, 8, 64), (1, 1, 64), (2, 4, 128)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_positions_far_below_zero(dtype, h, grp, d, far):
+    """Rows that attend nothing get zeros however far below zero their position is, in full tiles (8 heads) and beside other rows."""
+    a = setup_attention([9000, 4095, 10, 6500], [1, 1, 1, 1], h, grp, d, dtype, seed=3)
+    a[5][0], a[5][2] = far, far
+    for max_len in (9001, 1000):
+        got = check_attention(a, dtype, max_new=1, max_len=max_len, keys=9001)
+        assert float(got[0].abs().max()) == 0.0 and float(got[2].abs().max()) == 0.0
+    b = setup_attention([9000, 3, 2500, 1023], [70, 64, 130, 8], h, grp, d, dtype, seed=5, extra_rows=2)
+    b[5][:16] = far                                                          # whole tiles of the general form
+    b[5][40], b[5][200] = far, far
+    for kw in (dict(max_new=130, max_len=9070), dict(max_new=130, max_len=1500), dict()):
+        got = check_attention(b, dtype, cu_tok=b[6], keys=9070, **kw)
+        assert float(got[:16].abs().max()) == 0.0 and float(got[40].abs().max()) == 0.0
+    b[5][70:264] = far                                                       # all rows of two sequences
+    got = check_attention(b, dtype, cu_tok=b[6], keys=9070, max_new=130, max_len=9070)
+    assert float(got[70:264].abs().max()) == 0.0
