@@ -13,7 +13,8 @@
 //     to 2^-16 of the row's largest value (bf16 has 2^-9 of each), p vs to 2^-15 or 2^-16 of the largest p vs there has been (the
 //     output is rounded to 2^-9).  Products are exact, sums are 32-bit integers.
 //   fp32 rows: m16n8k16 on fp16, in which the integers are exact, q and p vs, relative to the same largest, split into a high and
-//     a low fp16 part, 22 bits, fp32 sums: fp32 accuracy.  A byte costs 1.25-1.5 instructions on its way there (xor the sign, byte-permute under 0x64
+//     a low fp16 part, 22 bits, fp32 sums: fp32 accuracy.  The largest p vs is brought near the top of fp16's range, so that parts
+//     become subnormal, good to 2^-38 of the largest and no more, only for weights that even many of cannot matter.  A byte costs 1.25-1.5 instructions on its way there (xor the sign, byte-permute under 0x64
 //     = 1024 + x, subtract), where I8 spends none on K and half of one on V, to bring four keys of a dim into one register.
 //
 // The kernel is to be bound by HBM: 2 head_dim bytes per cached position and kv head.  A block of threads takes one (row
@@ -78,6 +79,7 @@ __device__ __forceinline__ void mma16832(int (&c)[4], const uint32_t (&a)[4], ui
 // [-128, 127].  The sum with 1.5 * 2^23 + 128 leaves the integer, 128 up, in the low bits: its second byte is the high digit and
 // its first, sign flipped, the low one.
 constexpr float kDigits = 32512.f;
+constexpr float kSplitTop = 16384.f;   // what the largest weight of the fp16 form is brought to: its parts are then good to 2^-38 of it
 __device__ __forceinline__ uint32_t digit_bits(float x, float f) { return __float_as_uint(fmaf(x, f, 12583040.f)); }
 __device__ __forceinline__ void digits4(uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3, uint32_t& hi, uint32_t& lo) {
     const uint32_t a = __byte_perm(x0, x1, 0x5140), b = __byte_perm(x2, x3, 0x5140);      // low, low, high, high
@@ -352,7 +354,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
             w_run = w_new;
             // p of this step times these.  2^(m - w_run) in two halves: neither overflows beside a vs that is as far from 1.
             const float half_w = w_run == -INFINITY ? 0.f : exp2_fast(fminf(fmaxf(0.5f * (m_use - w_run), -126.f), 126.f));
-            const float k = I8 ? kDigits : 1.f, g0 = fminf(vs0 * half_w * k * half_w, 3e38f), g1 = fminf(vs1 * half_w * k * half_w, 3e38f);     // finite: a p of 0 stays 0
+            const float k = I8 ? kDigits : kSplitTop, g0 = fminf(vs0 * half_w * k * half_w, 3e38f), g1 = fminf(vs1 * half_w * k * half_w, 3e38f);     // finite: a p of 0 stays 0
             // a scale that is NaN shows by way of the sum: digits carry none, and g does not either
             if (vs0 != vs0 && kb <= pos) l_run = vs0;
             if (vs1 != vs1 && kb + kBlk8 <= pos) l_run = vs1;
@@ -471,7 +473,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     for (int j = 0; j < VB; ++j)
 #pragma unroll
         for (int e = 0; e < 2; ++e)                              // column 2t + e of column tile j is dim (2t + e) VB + j
-            so[(warp * kA8Rows + g) * OS + (2 * t + e) * VB + j] = (I8 ? fmaf((float)o[j][e], 256.f, (float)o[j][e + 2]) * (1.f / kDigits) : (float)o[j][e] + (float)o[j][e + 2]) * from_w * from_w;
+            so[(warp * kA8Rows + g) * OS + (2 * t + e) * VB + j] = (I8 ? fmaf((float)o[j][e], 256.f, (float)o[j][e + 2]) * (1.f / kDigits) : ((float)o[j][e] + (float)o[j][e + 2]) * (1.f / kSplitTop)) * from_w * from_w;
     __syncthreads();
     // eight dims per thread at a time: the four states joined in the order of the warps
     for (int x = tid; x < kA8Rows * HD / 8; x += kA8Threads) {
