@@ -10,11 +10,12 @@
 //
 // The integers are multiplied as they are (exact in fp16), scales act outside the products and cost nothing per element: with
 // c = scale log2(e) ks(block) and v = vs(block) / vr the weight is  w = p v = exp2(S c + (log2 v - m)),  one fma and one ex2, and
-// the softmax denominator sums w / v block by block.  vr is a power of two near the first vs, m the largest S c + log2 v so far: what
-// the attended values contribute, and not the loudest value of the cache, is what fp16's range is spent on.
-// w is rounded to fp16 (2^-11 of a weight; the output is rounded to bf16, 2^-8) and q, bf16 divided by a power of two, is
+// the softmax denominator sums w / v block by block.  vr is a power of two near the first vs, m the largest S c + log2 v so far less 7: what
+// the attended values contribute, and not the loudest value of the cache, is what fp16's range is spent on, all of it: the largest
+// weight is 2^7 or more, fp16 rounds one to 2^-11 of itself down to 2^-21 of the largest and drops it below 2^-32, so that what a hundred
+// thousand keys beside a strong one add up to is kept.  (The output is rounded to bf16, 2^-8.)  q, bf16 divided by a power of two, is
 // exact in fp16 down to 2^-16 of the row's largest value.  m does not follow every new
-// maximum but one that passes it by more than 8 (a factor of 256, which fp16 and the fp32 sums take): O in tensor memory is then rescaled, which is rare,
+// maximum but one that brings weights above 2^15: O in tensor memory is then rescaled, which is rare,
 // and so the exponentials need not wait for the maximum of their own step.
 //
 // What bounds it: 16 exponentials a clock and SM (1024 clocks for two tiles' step) against 1290 clocks of products at head_dim 128
@@ -38,7 +39,8 @@ constexpr int kT8Keys = kPage;                   // keys of a step: a page
 constexpr int kT8Blks = kT8Keys / kBlk8;         // scale blocks of a step
 constexpr int kT8Ring = 8;                       // steps whose scales are held
 constexpr int kT8Stages = 4;                     // widened K (and V) tiles
-constexpr float kT8Slack = 8.f;                  // log2 units that scores may pass m by
+constexpr float kT8Start = 7.f;                  // log2 of a row's largest weight when m is set
+constexpr float kT8Slack = 15.f;                 // log2 units that scores may pass m by: a weight is at most 2^15
 constexpr int kT8MaxSort = 64;                   // sequences up to which blocks order the tiles by their keys
 constexpr int kT8MaxCu = 1024;                   // sequences up to which a tile is looked for in shared memory
 
@@ -490,7 +492,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
                     mx = fmaxf(mx, fmaf(top, fmaxf(blk[b].x * row_f, 1e-37f), blk[b].y));
                 }
                 tc_wait_st();
-                if (i == 0) { m = mx; vr = vr_now; }
+                if (i == 0) { m = mx - kT8Start; vr = vr_now; }
             }
             // Weights against the m there is, and beside them their maximum, which the exponentials so need not wait for.  Where a row has
             // passed m by too much (in its first step, and rarely later), m moves and the step is done again: S is still there.
@@ -532,7 +534,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
                 }
                 const bool moves = mx > m + kT8Slack || (m == -INFINITY && mx > m);
                 if (!__any_sync(0xffffffffu, moves || vr_now != vr)) break;
-                const float m_new = moves ? mx : m;
+                const float m_new = moves ? mx - kT8Start : m;
                 const float corr = m == -INFINITY ? 0.f : exp2_fast(m - m_new);
                 l *= corr;
                 if (i > 0) {                                   // O as the products so far leave it: the last of them has to be done

@@ -103,3 +103,26 @@ def test_decode_with_a_strong_first_key(dtype, d, keys, spread, gap):
         for i in range(3):                                                   # rows of one length are one result
             same = got[i::3]
             assert torch.equal(same, same[:1].expand_as(same))
+
+
+@pytest.mark.parametrize("gap", [7.0, 10.6, 14.0, 17.0])
+@pytest.mark.parametrize("keys,spread", [(2048, 0.0), (32768, 0.0), (32768, 0.5), (131072, 0.0)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompts_with_a_strong_first_key(d, keys, spread, gap):
+    pages, scales = sink_cache(keys, 1, d, gap, spread, seed=keys)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for n in (160, 1):                                                       # sequences of the same pages: uncut, and cut where they are few
+        new = 130
+        table = torch.arange(pages.shape[0], **i32)[None].expand(n, -1).contiguous()
+        seq = torch.arange(n, **i32).repeat_interleave(new)
+        pos = (keys - new + torch.arange(new, **i32)).repeat(n)
+        cu = torch.arange(n + 1, **i32) * new
+        q = torch.ones(n * new, 1, d, dtype=torch.bfloat16, device="cuda")
+        if n > 1:
+            assert workspace(q, pages, scales, table, seq, pos, cu, new, keys) == 0
+        got = kv8.attention(q, pages, scales, table, seq, pos, cu, max_new=new, max_len=keys)
+        for t in (0, 5, 127, 128, 129):
+            want, tol = _bounds(q[t:t + 1], pages, scales, pos[t:t + 1], torch.bfloat16, True)
+            err = (got[t:t + 1].double() - want).abs()
+            assert bool((err <= tol).all()), (n, t, float((err / tol).max()), float((err / want.abs().clamp(min=1e-3)).max()))
+        assert torch.equal(got, got[:new].repeat(n, 1, 1))
