@@ -321,9 +321,10 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
             if (vr == 0.f && top > 0.f) vr = pow2_above(fminf(top, 1.7e38f));
             const float v0 = vr > 0.f ? vs / vr : (vs == 0.f ? 1.f : vs);
             // Within 2^-60 and 2^100: at the lower end fp16 takes a weight for 0 beside any other, the sum does not; the upper one is
-            // out of reach for values that one model made.
-            const float v = v0 != v0 ? v0 : fminf(fmaxf(v0, 8.67361738e-19f), 1.26765060e30f);
-            const float4 f = counts ? make_float4(ks * fabsf(a.scale) * 1.4426950408889634f, ks == ks ? log2f(v) : ks, 1.f / v, 0.f) : make_float4(0.f, -INFINITY, 0.f, 0.f);
+            // out of reach for values that one model made.  A scale that is not finite makes the weights of its block NaN, and
+            // nothing else: the other factors also meet rows that stand before it.
+            const float v = fminf(fmaxf(v0, 8.67361738e-19f), 1.26765060e30f), odd = (ks - ks) + (vs - vs);       // 0 or NaN
+            const float4 f = counts ? make_float4(ks * fabsf(a.scale) * 1.4426950408889634f, log2f(v) + odd, 1.f / v, 0.f) : make_float4(0.f, -INFINITY, 0.f, 0.f);
             // the K of a step is free once S is done, which was asked for when the softmax had ended the step two before: with the
             // K of step i - stages free it is done with i - stages - 2, far behind the ring's length
             if (i >= kT8Stages) ok = __all_sync(0xffffffffu, wait8(B(K_FREE + i % kT8Stages), parity(i - kT8Stages)));
@@ -508,11 +509,11 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
                 l_add = 0.f;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
+                    // c stays above zero so that -inf stays -inf; a block behind the row does not count, whatever it holds: S is -inf there,
+                    // and f.y, which alone may be NaN, is not used
                     const float4 f = blk[b];
-                    // c stays above zero so that -inf stays -inf (a block's factor that is NaN comes by f.y); a block behind the row
-                    // does not count, whatever it holds: its factors, which may be infinite or NaN, are not used in the maximum, the weights or the sum
                     const bool behind = k0 + b * 16 > open;
-                    const float c = behind ? 1e-37f : fmaxf(f.x * row_f, 1e-37f), d = behind ? -INFINITY : f.y - m_use;
+                    const float c = fmaxf(f.x * row_f, 1e-37f), d = behind ? -INFINITY : f.y - m_use;
                     float t4[2] = {__uint_as_float(sv[b * 16]), __uint_as_float(sv[b * 16 + 1])};
 #pragma unroll
                     for (int j = 2; j < 16; j += 4) {
@@ -530,7 +531,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
                         pk[b * 8 + j / 2] = pack_half(w0, w1);
                     }
                     const float2 s2 = unpair2(sum);
-                    l_add = fmaf(s2.x + s2.y, behind ? 0.f : f.z, l_add);
+                    l_add = fmaf(s2.x + s2.y, f.z, l_add);
                 }
                 const bool moves = mx > m + kT8Slack || (m == -INFINITY && mx > m);
                 if (!__any_sync(0xffffffffu, moves || vr_now != vr)) break;
