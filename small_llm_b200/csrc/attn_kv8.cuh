@@ -7,14 +7,15 @@
 // integer product, so the products run on the integers themselves: mma.sync with eight query rows (tokens x heads that share
 // a kv head) as its rows 0..7, and what the 8 or 11 bits of an operand leave out of them as its rows 8..15, so that both parts
 // come out in one thread and are added there, at no more matrix instructions than one row costs.  q is first divided by a power
-// of two so that its largest value is in [0.5, 1); the largest p vs so far is carried beside the running maximum m, so that what the
-// attended values leave room for, and not the loudest value of the cache, sets the precision.  Two forms:
+// of two so that its largest value is in [0.5, 1).  The products with V are of one unit of 32 keys at a time: its weights p vs are taken
+// relative to their own largest, and the unit's sum is added, with that factor, to an fp32 accumulator relative to m.  So the
+// precision of a weight is that of its unit: neither the loudest value of the cache, nor a strong key (an attention sink) elsewhere
+// in it, takes bits from what many small weights add up to.  Two forms:
 //   bf16 rows (I8): m16n8k32 on int8, the cache's bytes as they are.  q and p vs become two base-256 digits, 16 bits in all: q
-//     to 2^-16 of the row's largest value (bf16 has 2^-9 of each), p vs to 2^-15 or 2^-16 of the largest p vs there has been (the
-//     output is rounded to 2^-9).  Products are exact, sums are 32-bit integers.
-//   fp32 rows: m16n8k16 on fp16, in which the integers are exact, q and p vs, relative to the same largest, split into a high and
-//     a low fp16 part, 22 bits, fp32 sums: fp32 accuracy.  The largest p vs is brought near the top of fp16's range, so that parts
-//     become subnormal, good to 2^-38 of the largest and no more, only for weights that even many of cannot matter.  A byte costs 1.25-1.5 instructions on its way there (xor the sign, byte-permute under 0x64
+//     to 2^-17 of the row's largest value (bf16 has 2^-9 of each), p vs to 2^-16 of the unit's largest (the
+//     output is rounded to 2^-9).  Products and a unit's sums are exact, in 32-bit integers.
+//   fp32 rows: m16n8k16 on fp16, in which the integers are exact, q and p vs split into a high and a low fp16 part, 22 bits (p vs to 2^-39
+//     of the unit's largest at least), fp32 sums: fp32 accuracy.  A byte costs 1.25-1.5 instructions on its way there (xor the sign, byte-permute under 0x64
 //     = 1024 + x, subtract), where I8 spends none on K and half of one on V, to bring four keys of a dim into one register.
 //
 // The kernel is to be bound by HBM: 2 head_dim bytes per cached position and kv head.  A block of threads takes one (row
@@ -79,7 +80,7 @@ __device__ __forceinline__ void mma16832(int (&c)[4], const uint32_t (&a)[4], ui
 // [-128, 127].  The sum with 1.5 * 2^23 + 128 leaves the integer, 128 up, in the low bits: its second byte is the high digit and
 // its first, sign flipped, the low one.
 constexpr float kDigits = 32512.f;
-constexpr float kSplitTop = 16384.f;   // what the largest weight of the fp16 form is brought to: its parts are then good to 2^-38 of it
+constexpr float kSplitTop = 16384.f;   // what a unit's largest weight of the fp16 form is brought to: its parts are then good to 2^-39 of it
 __device__ __forceinline__ uint32_t digit_bits(float x, float f) { return __float_as_uint(fmaf(x, f, 12583040.f)); }
 __device__ __forceinline__ void digits4(uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3, uint32_t& hi, uint32_t& lo) {
     const uint32_t a = __byte_perm(x0, x1, 0x5140), b = __byte_perm(x2, x3, 0x5140);      // low, low, high, high
@@ -106,6 +107,11 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 // smallest power of two >= x, for 0 <= x < infinity (0 for 0)
@@ -249,10 +255,10 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     }
 
     using Acc = typename std::conditional<I8, int, float>::type;
-    Acc o[VB][4];
+    float o[VB][2];
 #pragma unroll
-    for (int j = 0; j < VB; ++j) { o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0; }
-    float m_run = -INFINITY, l_run = 0.f, w_run = -INFINITY;
+    for (int j = 0; j < VB; ++j) o[j][0] = o[j][1] = 0.f;
+    float m_run = -INFINITY, l_run = 0.f;
 
     const int n_units = keys > 0 ? (keys + kA8Unit - 1) / kA8Unit : 0;
     const int mine = n_units > warp ? (n_units - warp + kA8Warps - 1) / kA8Warps : 0;
@@ -340,32 +346,30 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             const float m_new = fmaxf(m_run, mx);
             const float m_use = m_new == -INFINITY ? 0.f : m_new;
-            l_run *= exp2_fast(m_run - m_use);
-            m_run = m_new;
+            if (__any_sync(0xffffffffu, m_new != m_run)) {
+                const float corr = exp2_fast(m_run - m_use);
+                m_run = m_new;
+                l_run *= corr;
+#pragma unroll
+                for (int j = 0; j < VB; ++j) { o[j][0] *= corr; o[j][1] *= corr; }
+            }
             // the second block of a unit may lie behind the last position: its scale is another owner's then and does not count
             const float vs0 = scl[4], vs1 = kb + kBlk8 <= last ? scl[5] : 0.f;
-            // The weights of the product with V are p vs relative to the largest there has been, 2^w_run.  Digits must not pass 1, so w_run
-            // moves one further than it has to, and so less often.
             float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1])) + __log2f(vs0), fmaxf(fmaxf(sc[2][0], sc[2][1]), fmaxf(sc[3][0], sc[3][1])) + __log2f(vs1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float w_new = top > w_run ? top + 1.f : w_run;
-            const float corr = w_new == w_run ? 1.f : exp2_fast(w_run - w_new);          // equal: also where both are -inf
-            w_run = w_new;
-            // p of this step times these.  2^(m - w_run) in two halves: neither overflows beside a vs that is as far from 1.
-            const float half_w = w_run == -INFINITY ? 0.f : exp2_fast(fminf(fmaxf(0.5f * (m_use - w_run), -126.f), 126.f));
-            const float k = I8 ? kDigits : kSplitTop, g0 = fminf(vs0 * half_w * k * half_w, 3e38f), g1 = fminf(vs1 * half_w * k * half_w, 3e38f);     // finite: a p of 0 stays 0
-            // a scale that is NaN shows by way of the sum: digits carry none, and g does not either
-            if (vs0 != vs0 && kb <= pos) l_run = vs0;
-            if (vs1 != vs1 && kb + kBlk8 <= pos) l_run = vs1;
-            if (__any_sync(0xffffffffu, corr != 1.f)) {
+            // The unit's weights are p times these, k times what they are relative to its largest p vs, 2^top; its sum counts unit_f times.
+            // Within 2^-120: what is below that adds nothing to a number that fp32 holds.
+            constexpr float k = I8 ? kDigits : kSplitTop;
+            const float unit_top = exp2_fast(fminf(fmaxf(top - m_use, -120.f), 126.f)), r = rcp_fast(unit_top), unit_f = unit_top * (1.f / k);
+            const float g0 = fminf(vs0 * r * k, 3e38f), g1 = fminf(vs1 * r * k, 3e38f);   // 0 for a scale of 0, and finite: a p of 0 stays 0
+            // a scale that is not finite shows by way of the sum: digits carry none, and g does not either
+            if (!(vs0 < INFINITY) && kb <= pos) l_run = __uint_as_float(0x7fffffffu);
+            if (!(vs1 < INFINITY) && kb + kBlk8 <= pos) l_run = __uint_as_float(0x7fffffffu);
+            auto add = [&](int j, const Acc (&c)[4]) {           // a unit's product of column tile j
 #pragma unroll
-                for (int j = 0; j < VB; ++j)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if constexpr (I8) o[j][k] = __float2int_rn((float)o[j][k] * corr);       // half a unit off: 2^-16 of one key's weight
-                        else o[j][k] *= corr;
-            }
+                for (int e = 0; e < 2; ++e) o[j][e] = fmaf(I8 ? (float)((int)c[e] * 256 + (int)c[e + 2]) : (float)c[e] + (float)c[e + 2], unit_f, o[j][e]);
+            };
             if constexpr (I8) {
                 uint32_t pa[4], x[8];
 #pragma unroll
@@ -401,56 +405,49 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
                         b[h][2] = __byte_perm(r1, r3, 0x5410); b[h][3] = __byte_perm(r1, r3, 0x7632);
                     }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) mma16832(o[4 * w + k], pa, b[0][k], b[1][k]);
+                    for (int k = 0; k < 4; ++k) { int c[4] = {0, 0, 0, 0}; mma16832(c, pa, b[0][k], b[1][k]); add(4 * w + k, c); }
                 }
             } else {
+                uint32_t pa[2][4];
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                const float vf = kk ? g1 : g0;
-                uint32_t pa[4];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < 4; ++h) {
                     float p[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const int key = kb + (2 * kk + h) * 8 + ((2 * t + e) ^ (t >> 1));
-                        p[e] = exp2_fast(sc[2 * kk + h][e] - m_use);
+                        const int key = kb + h * 8 + ((2 * t + e) ^ (t >> 1));
+                        p[e] = exp2_fast(sc[h][e] - m_use);
                         l_run += p[e];
-                        p[e] = key <= pos ? p[e] * vf : 0.f;
+                        p[e] = key <= pos ? p[e] * (h >> 1 ? g1 : g0) : 0.f;
                     }
-                    split2(p[0], p[1], pa[2 * h], pa[2 * h + 1]);
+                    split2(p[0], p[1], pa[h >> 1][2 * (h & 1)], pa[h >> 1][2 * (h & 1) + 1]);
                 }
-                // V rows of keys (2t, 2t + 1) and (2t + 8, 2t + 9) of this block, as permuted above
-                const unsigned char* row = sv + (kk * kBlk8) * HD + g * VB;
+                // V rows of keys (2t, 2t + 1) and (2t + 8, 2t + 9) of each block, as permuted above
+                constexpr int NW = (VB + 3) / 4, NB = VB < 4 ? VB : 4;               // head_dim 16: two bytes of each row
                 const int e0 = (2 * t) ^ (t >> 1), e1 = (2 * t + 1) ^ (t >> 1);
-                if constexpr (VB >= 4) {
-                    constexpr int NW = VB / 4;
-                    uint32_t v[4][NW];
+                uint32_t v[8][NW];
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const unsigned char* src = row + ((x & 1 ? e1 : e0) + (x >> 1) * 8) * HD;
-                        if constexpr (NW == 4) *reinterpret_cast<uint4*>(v[x]) = *reinterpret_cast<const uint4*>(src);
-                        else if constexpr (NW == 2) *reinterpret_cast<uint2*>(v[x]) = *reinterpret_cast<const uint2*>(src);
-                        else v[x][0] = *reinterpret_cast<const uint32_t*>(src);
-                    }
-#pragma unroll
-                    for (int w = 0; w < NW; ++w) {
-                        const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140) ^ 0x80808080u, a1 = __byte_perm(v[0][w], v[1][w], 0x7362) ^ 0x80808080u;
-                        const uint32_t b0 = __byte_perm(v[2][w], v[3][w], 0x5140) ^ 0x80808080u, b1 = __byte_perm(v[2][w], v[3][w], 0x7362) ^ 0x80808080u;
-                        mma16816(o[4 * w], pa, halves(a0, 0x4140), halves(b0, 0x4140));
-                        mma16816(o[4 * w + 1], pa, halves(a0, 0x4342), halves(b0, 0x4342));
-                        mma16816(o[4 * w + 2], pa, halves(a1, 0x4140), halves(b1, 0x4140));
-                        mma16816(o[4 * w + 3], pa, halves(a1, 0x4342), halves(b1, 0x4342));
-                    }
-                } else {                                         // head_dim 16: two bytes of each row
-                    uint32_t v[4];
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) v[x] = *reinterpret_cast<const uint16_t*>(row + ((x & 1 ? e1 : e0) + (x >> 1) * 8) * HD);
-                    const uint32_t a0 = __byte_perm(v[0], v[1], 0x5140) ^ 0x80808080u, b0 = __byte_perm(v[2], v[3], 0x5140) ^ 0x80808080u;
-                    mma16816(o[0], pa, halves(a0, 0x4140), halves(b0, 0x4140));
-                    mma16816(o[1], pa, halves(a0, 0x4342), halves(b0, 0x4342));
+                for (int x = 0; x < 8; ++x) {
+                    const unsigned char* src = sv + ((x & 1 ? e1 : e0) + (x >> 1) * 8) * HD + g * VB;
+                    if constexpr (VB == 16) *reinterpret_cast<uint4*>(v[x]) = *reinterpret_cast<const uint4*>(src);
+                    else if constexpr (VB == 8) *reinterpret_cast<uint2*>(v[x]) = *reinterpret_cast<const uint2*>(src);
+                    else if constexpr (VB == 4) v[x][0] = *reinterpret_cast<const uint32_t*>(src);
+                    else v[x][0] = *reinterpret_cast<const uint16_t*>(src);
                 }
-            }
+#pragma unroll
+                for (int w = 0; w < NW; ++w)
+#pragma unroll
+                    for (int y = 0; y < NB; y += 2) {                    // two dims at a time
+                        float c[2][4] = {};
+#pragma unroll
+                        for (int kk = 0; kk < 2; ++kk) {
+                            const uint32_t a2 = __byte_perm(v[4 * kk][w], v[4 * kk + 1][w], y ? 0x7362 : 0x5140) ^ 0x80808080u;
+                            const uint32_t b2 = __byte_perm(v[4 * kk + 2][w], v[4 * kk + 3][w], y ? 0x7362 : 0x5140) ^ 0x80808080u;
+                            mma16816(c[0], pa[kk], halves(a2, 0x4140), halves(b2, 0x4140));
+                            mma16816(c[1], pa[kk], halves(a2, 0x4342), halves(b2, 0x4342));
+                        }
+                        add(4 * w + y, c[0]);
+                        add(4 * w + y + 1, c[1]);
+                    }
             }
             __syncwarp();                                        // every lane is done with stage s
         }
@@ -468,12 +465,11 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     constexpr int OS = HD + 4;                                   // floats per row: rows start in different banks
     static_assert((size_t)kA8Warps * kA8Rows * OS * 4 <= attn8_smem<HD>(), "the joined states fit the stages");
     float* so = reinterpret_cast<float*>(smem_raw);
-    const float from_w = w_run == -INFINITY ? 0.f : exp2_fast(fminf(fmaxf(0.5f * (w_run - m_run), -126.f), 126.f));      // back to p vs, by halves as well
 #pragma unroll
     for (int j = 0; j < VB; ++j)
 #pragma unroll
         for (int e = 0; e < 2; ++e)                              // column 2t + e of column tile j is dim (2t + e) VB + j
-            so[(warp * kA8Rows + g) * OS + (2 * t + e) * VB + j] = (I8 ? fmaf((float)o[j][e], 256.f, (float)o[j][e + 2]) * (1.f / kDigits) : ((float)o[j][e] + (float)o[j][e + 2]) * (1.f / kSplitTop)) * from_w * from_w;
+            so[(warp * kA8Rows + g) * OS + (2 * t + e) * VB + j] = o[j][e];
     __syncthreads();
     // eight dims per thread at a time: the four states joined in the order of the warps
     for (int x = tid; x < kA8Rows * HD / 8; x += kA8Threads) {

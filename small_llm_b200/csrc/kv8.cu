@@ -251,10 +251,8 @@ int attn_form(const Plan& p, int dev, void* stream) {
 }
 template <typename T, int HD>
 int attn_hd(const Plan& p, int dev, void* stream) {
-    // The integer form: bf16 rows, and no more keys per warp than its 32-bit sums hold whatever they are (2^17 products of 127 * 127).
-    if constexpr (std::is_same<T, __nv_bfloat16>::value && HD >= 32)
-        if ((long long)p.a.width * kPage <= (long long)kA8Warps << 17) return p.a.cluster ? attn_form<T, HD, true, true>(p, dev, stream) : attn_form<T, HD, true, false>(p, dev, stream);
-    return p.a.cluster ? attn_form<T, HD, false, true>(p, dev, stream) : attn_form<T, HD, false, false>(p, dev, stream);
+    constexpr bool i8 = std::is_same<T, __nv_bfloat16>::value && HD >= 32;           // the integer form: bf16 rows
+    return p.a.cluster ? attn_form<T, HD, i8, true>(p, dev, stream) : attn_form<T, HD, i8, false>(p, dev, stream);
 }
 template <int HD, int NT>
 int attn_tc(const Plan& p, int dev, void* stream) {

@@ -30,3 +30,15 @@ def test_positions_far_below_zero(dtype, h, grp, d, far):
     b[5][70:264] = far                                                       # all rows of two sequences
     got = check_attention(b, dtype, cu_tok=b[6], keys=9070, max_new=130, max_len=9070)
     assert float(got[70:264].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("h,grp,d", [(2, 1, 32), (2, 2, 64), (1, 4, 128)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_tables_of_many_pages(dtype, h, grp, d):
+    """A table wider than 8192 pages, most of it not in use, with lengths known and not known; integers down to -128."""
+    a = setup_attention([700, 20, 4000], [1, 3, 40], h, grp, d, dtype, seed=d, width_more=9000)
+    q, pages, scales, table, seq, pos, cu = a
+    pages.masked_fill_(pages == -127, -128)
+    assert table.shape[1] > 8192
+    for kw in (dict(max_new=1, max_len=4040), dict(max_new=1), dict(cu_tok=cu, max_new=40, max_len=4040), dict(cu_tok=cu)):
+        check_attention(a, dtype, keys=4040, **kw)

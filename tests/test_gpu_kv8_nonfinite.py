@@ -56,3 +56,16 @@ def test_prompts_in_chunks_with_a_block_that_is_not_finite(h, grp, d, which):
         bad = torch.isnan(got).any(-1)[:, :grp].all(1).cpu()
         assert bad.tolist() == [i < 70 and i not in (3, 10) for i in range(len(seq))]
         assert float(got[3].abs().max()) == 0.0 and float(got[80].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("dtype,d,kw", [(torch.float32, 64, dict(max_new=1)), (torch.bfloat16, 64, dict(max_new=1)), (torch.bfloat16, 16, dict(max_new=1)), (torch.bfloat16, 128, dict()),
+                                        (torch.float32, 128, dict())])
+def test_infinite_values_show_where_they_are_attended(dtype, d, kw, which):
+    q, pages, scales, table, seq, pos, cu = setup_attention([0], [150], 2, 2, d, dtype, seed=80)
+    scales[int(table[0, 1]), 1, which, 2] = math.inf                         # keys 96 .. 111, kv head 1
+    got = kv8.attention(q, pages, scales, table, seq, pos, None if kw else cu, max_len=150, **kw)
+    odd = ~torch.isfinite(got).all(-1)
+    assert not bool(odd[:96].any()) and not bool(odd[:, :2].any())
+    # K: scores without end of both signs, of which one takes everything; all of one sign downwards may leave the rest
+    assert bool(odd[111:, 2:].all()) if which else float(odd[111:, 2:].float().mean()) > 0.9

@@ -83,7 +83,7 @@ def workspace(q, pages, scales, table, seq, pos, cu, max_new, max_len):
 @pytest.mark.parametrize("gap", [7.0, 10.6, 14.0, 17.0])
 @pytest.mark.parametrize("keys,spread", [(2048, 0.0), (8192, 1.0), (32768, 0.0), (32768, 0.5)])
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("dtype", [torch.float32])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_decode_with_a_strong_first_key(dtype, d, keys, spread, gap):
     """Enough sequences (of the same pages) that the keys of a row are not cut, and a few, which are."""
     h = 2
@@ -126,3 +126,15 @@ def test_prompts_with_a_strong_first_key(d, keys, spread, gap):
             err = (got[t:t + 1].double() - want).abs()
             assert bool((err <= tol).all()), (n, t, float((err / tol).max()), float((err / want.abs().clamp(min=1e-3)).max()))
         assert torch.equal(got, got[:new].repeat(n, 1, 1))
+
+
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_values_near_the_largest_number(dtype, d):
+    """Two keys of one score whose values are 2^126 and less: their mean, not infinity."""
+    pages, scales = kv8.empty_cache(1, 1, d)
+    pages[0, 0, 1, 0], pages[0, 0, 1, 1] = 127, 64
+    scales[0, 0, 1, 0] = 2.0 ** 119
+    i32 = dict(dtype=torch.int32, device="cuda")
+    got = kv8.attention(torch.ones(1, 1, d, dtype=dtype, device="cuda"), pages, scales, torch.zeros(1, 1, **i32), torch.zeros(1, **i32), torch.ones(1, **i32), max_new=1)
+    assert bool(((got.double() / (95.5 * 2.0 ** 119) - 1).abs() <= (2.0 ** -8 + 2.0 ** -15 if dtype == torch.bfloat16 else 2.0 ** -20)).all())
