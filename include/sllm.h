@@ -298,7 +298,9 @@ int sllm_k_kv8_read(const sllm_kv8_layer* c, const sllm_kv8_rows* r, void* strea
  * (its own included: append first).  n_heads is a multiple of kv_heads; query head h attends kv head h / (n_heads / kv_heads).
  * Softmax in fp32 and the integers of the cache exactly; fp32 rows keep fp32 accuracy.
  * A token with tok_seq outside 0 .. n_seq - 1 is skipped, its output row left as it was; one with tok_pos < 0 gets zeros.  A
- * page outside the pool is not attended, and *status (when given, an int32 that the call never clears) becomes SLLM_ERR_INVALID.
+ * page outside the pool is not attended.  *status (when given, an int32 that the call never clears) becomes SLLM_ERR_INVALID when
+ * there was one, and SLLM_ERR_DEVICE_WAIT when a bounded wait of a kernel gave up.  The rows that such a wait concerns are NaN, with
+ * or without a status.
  * max_new: the most entries that one sequence has; max_len: the most positions that one has.  They choose between kernels and how
  * the keys are cut; 0 = not known; a wrong value costs time, not results.  cu_tok (NULL allowed: then every token is taken
  * alone) says that entries cu_tok[i] .. cu_tok[i + 1] - 1 are sequence i's, with the table's row i; it is used when max_new != 1. */

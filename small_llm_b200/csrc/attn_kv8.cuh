@@ -453,15 +453,13 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
         }
         if (i + ST < mine) issue(i + ST);
     }
-    if (!ok) { s_ok = 0; if (a.status) atomicExch(a.status, 5); }
+    if (!ok) { s_ok = 0; l_run = __uint_as_float(0x7fffffffu); if (a.status) atomicExch(a.status, 5); }      // the tile's rows become NaN
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
     if (t == 0) { s_m[warp][g] = m_run; s_l[warp][g] = l_run; }
     __syncthreads();                                             // every warp is done with its stages: their memory is used again
-    if (!s_ok) {                                                 // let copies in flight land before shared memory is released
+    if (!s_ok)                                                   // let copies in flight land before shared memory is used again and released
         for (int i = 0; i < 32; ++i) __nanosleep(16384);
-        if (!CL) return;                                  // the cluster's other blocks are at its barriers
-    }
     constexpr int OS = HD + 4;                                   // floats per row: rows start in different banks
     static_assert((size_t)kA8Warps * kA8Rows * OS * 4 <= attn8_smem<HD>(), "the joined states fit the stages");
     float* so = reinterpret_cast<float*>(smem_raw);

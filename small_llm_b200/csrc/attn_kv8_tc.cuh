@@ -27,7 +27,7 @@
 // block at head_dim 128 (a step of 3100 tokens 89 us against 77 then).
 // 7.4 thousand prompt tokens of ten heads of 64 take 44 us, half of it the blocks' beginnings and ends (eight steps on average).
 // Where there are few blocks for the GPU the keys are cut into chunks (grid z), whose states the general form's second kernel joins.
-// Every wait is bounded; on expiry the block sets *status, frees its tensor memory and returns.
+// Every wait is bounded; on expiry the block sets *status, gives its rows NaN, frees its tensor memory and returns.
 #pragma once
 #include "attn_kv8.cuh"
 #include "tc_ptx.cuh"
@@ -573,23 +573,22 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
         if (my_steps > 0 && ok) ok = wait8(B(PV_DONE + 2 * tile + ((my_steps - 1) & 1)), ((my_steps - 1) >> 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
-        if (ok) {
-            const bool whole = own_chunks <= 1;
-            const float f = whole ? (l == 0.f ? 0.f : vr / l) : vr;
-            const long long part = ((long long)row_tok * a.n_heads + row_head) * a.n_chunks + chunk;
-            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (row_tok >= 0 ? (long long)row_tok * a.out_stride + row_head * HD : 0);
-            if (!whole && row_tok >= 0) { a.part_ml[part * 2] = m; a.part_ml[part * 2 + 1] = l; }
+        if (!ok) l = __uint_as_float(0x7fffffffu);             // a wait ran out: the rows become NaN
+        const bool whole = own_chunks <= 1;
+        const float f = whole ? (l == 0.f ? 0.f : vr / l) : l == l ? vr : l;
+        const long long part = ((long long)row_tok * a.n_heads + row_head) * a.n_chunks + chunk;
+        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (row_tok >= 0 ? (long long)row_tok * a.out_stride + row_head * HD : 0);
+        if (!whole && row_tok >= 0) { a.part_ml[part * 2] = m; a.part_ml[part * 2 + 1] = l; }
 #pragma unroll
-            for (int h = 0; h < HD / 16; ++h) {
-                uint32_t o[16];
-                if (my_steps > 0) tc_ld16(o_at + h * 16, o);
-                float x[16];
+        for (int h = 0; h < HD / 16; ++h) {
+            uint32_t o[16];
+            if (my_steps > 0) tc_ld16(o_at + h * 16, o);
+            float x[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] = l == 0.f || my_steps == 0 ? 0.f : __uint_as_float(o[j]) * f;
-                if (row_tok < 0) continue;
-                if (whole) { store8(dst + h * 16, a.wide, x); store8(dst + h * 16 + 8, a.wide, x + 8); }
-                else { store8(a.part + part * HD + h * 16, true, x); store8(a.part + part * HD + h * 16 + 8, true, x + 8); }
-            }
+            for (int j = 0; j < 16; ++j) x[j] = l == 0.f || my_steps == 0 ? 0.f : __uint_as_float(o[j]) * f;
+            if (row_tok < 0) continue;
+            if (whole) { store8(dst + h * 16, a.wide, x); store8(dst + h * 16 + 8, a.wide, x + 8); }
+            else { store8(a.part + part * HD + h * 16, true, x); store8(a.part + part * HD + h * 16 + 8, true, x + 8); }
         }
     }
     if (!ok && a.status) atomicExch(a.status, 5);

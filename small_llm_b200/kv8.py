@@ -167,7 +167,9 @@ def attention(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, table:
 
     Token t attends positions 0 .. tok_pos[t] of sequence tok_seq[t] (int32 [n_tok]) through table int32 [n_seq, width].  max_new and
     max_len are the most tokens a sequence has in the list and the most positions any has: they choose how the work is cut
-    (0: not known).  Rows of tokens with tok_seq < 0 are left as they are, so give `out` where a list is padded."""
+    (0: not known).  Rows of tokens with tok_seq < 0 are left as they are, so give `out` where a list is padded.  status int32 [1]
+    takes the SLLM_ERR_* code of what the kernels find: a page outside the pool (it is not attended), a wait that gave up (the rows
+    are NaN)."""
     c, dev, h, d = _layer(pages, scales)
     _need(q.dim() == 3 and table.dim() == 2, "q must be [n_tok, n_heads, head_dim], table [n_seq, width]")
     n, heads = q.shape[0], q.shape[1]
@@ -214,7 +216,8 @@ class PagedCache:
     tensor that the captured step() was given, and the rows into the captured k, v and q, before each replay.
 
     A step that needs more pages or entries than there are, or a length above max_len, changes nothing and leaves empty lists:
-    status() says so (0, or the SLLM_ERR_* code), at the cost of a wait for the GPU, and the next step starts from the lengths before."""
+    status() says so (0, or the SLLM_ERR_* code), at the cost of a wait for the GPU, and the next step starts from the lengths before.
+    status() also says what attention() found (a page outside the pool, a wait that gave up)."""
 
     def __init__(self, n_layers: int, n_seqs: int, n_pages: int, kv_heads: int, head_dim: int, max_len: int, max_tok: int, device="cuda"):
         _need(n_layers > 0 and 0 < n_seqs <= MAX_SEQS and n_pages > 0 and max_len > 0 and max_tok > 0, f"counts must be positive, n_seqs at most {MAX_SEQS}")
@@ -229,6 +232,7 @@ class PagedCache:
         self.cu_tok = torch.zeros(n_seqs + 1, **i32)
         self.tok_seq, self.tok_pos = torch.full((max_tok,), -1, **i32), torch.full((max_tok,), -1, **i32)
         self.slot_map = torch.full((max_tok,), -1, dtype=_I64, device=dev)
+        self._found = torch.zeros(1, **i32)                  # what attention() found
 
     def step(self, len_after: torch.Tensor) -> None:
         """Moves every sequence to len_after (int32 [n_seqs] on the cache's device; 0 = it has ended) and makes the step's lists."""
@@ -244,15 +248,20 @@ class PagedCache:
     def attention(self, layer: int, q: torch.Tensor, *, max_new: int = 0, max_len: int = 0, scale: float | None = None, out: torch.Tensor | None = None,
                   status: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of the step's queries [max_tok, n_heads, head_dim] over a layer.  Rows behind the list's last are left as they
-        are in `out`, and zeros where it is not given."""
+        are in `out`, and zeros where it is not given.  What the kernels find goes to `status`, or where that is not given to status()."""
         if out is None:
             out = torch.zeros_like(q, memory_format=torch.contiguous_format)
         return attention(q, *self.layers[layer], self.table, self.tok_seq, self.tok_pos, self.cu_tok, max_new=max_new, max_len=max_len or self.max_len, scale=scale,
-                         out=out, status=status)
+                         out=out, status=self._found if status is None else status)
 
     def status(self) -> int:
-        """0, or the code of the last step's refusal."""
-        return int(self._pool[1, 3])
+        """The code of the last step's refusal, or else of what attention() has found since status() last said so, or else 0."""
+        code = int(self._pool[1, 3])
+        if code == 0:
+            code = int(self._found)
+            if code:
+                self._found.zero_()
+        return code
 
     def free_pages(self) -> int:
         return int(self._pool[0, 1])

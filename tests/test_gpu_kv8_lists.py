@@ -42,3 +42,18 @@ def test_tables_of_many_pages(dtype, h, grp, d):
     assert table.shape[1] > 8192
     for kw in (dict(max_new=1, max_len=4040), dict(max_new=1), dict(cu_tok=cu, max_new=40, max_len=4040), dict(cu_tok=cu)):
         check_attention(a, dtype, keys=4040, **kw)
+
+
+def test_paged_cache_says_what_attention_found():
+    cache = kv8.PagedCache(1, 2, 8, 2, 64, max_len=200, max_tok=130)
+    cache.step(torch.tensor([100, 30], dtype=torch.int32, device="cuda"))
+    x = torch.randn(130, 2, 64, device="cuda")
+    cache.append(0, x, x)
+    cache.attention(0, x)
+    assert cache.status() == 0
+    cache.table[0, 0] = 8                                                    # no such page
+    cache.attention(0, x)
+    assert cache.status() == 1 and cache.status() == 0                       # said once
+    mine = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cache.attention(0, x, status=mine)
+    assert int(mine) == 1 and cache.status() == 0
