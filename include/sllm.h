@@ -303,7 +303,8 @@ int sllm_k_kv8_read(const sllm_kv8_layer* c, const sllm_kv8_rows* r, void* strea
  * or without a status.
  * max_new: the most entries that one sequence has; max_len: the most positions that one has.  They choose between kernels and how
  * the keys are cut; 0 = not known; a wrong value costs time, not results.  cu_tok (NULL allowed: then every token is taken
- * alone) says that entries cu_tok[i] .. cu_tok[i + 1] - 1 are sequence i's, with the table's row i; it is used when max_new != 1. */
+ * alone) says that entries cu_tok[i] .. cu_tok[i + 1] - 1 are sequence i's, with the table's row i; it is used when max_new != 1, and
+ * entries whose tok_seq is not i are then skipped as well. */
 typedef struct {
     const void* q;                            /* [n_tok], rows of n_heads * head_dim elements                      */
     void* out;                                /* the same; may not overlap q                                       */

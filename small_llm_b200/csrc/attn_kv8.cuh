@@ -178,6 +178,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     __shared__ float s_cm[CL ? kA8Rows : 1], s_cl[CL ? kA8Rows : 1];
     __shared__ __align__(16) float s_co[CL ? kA8Rows : 1][CL ? HD : 4];      // the block's joined state, for the cluster
     __shared__ int s_ok;
+    __shared__ unsigned s_live;                  // bit 4 r: row r is somebody's
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     if (tid == 0) {
@@ -197,7 +198,10 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     const int chunk = blockIdx.z;
     // this lane's row
     const int r_tok = g / a.rows_heads, r_head = ht * a.rows_heads + g % a.rows_heads;
-    const bool row_ok = r_tok < n && r_head < a.group;
+    // a list's entry in a sequence's place that does not say so is skipped (without cu_tok the sequence is its own)
+    const bool row_ok = r_tok < n && r_head < a.group && (!a.cu_tok || a.tok_seq[t0 + r_tok] == seq);
+    const unsigned rows = __ballot_sync(0xffffffffu, row_ok);
+    if (tid == 0) s_live = rows;
     const int pos = row_ok ? max(min(a.tok_pos[t0 + r_tok], a.width * kPage - 1), -1) : -1;      // width * 64 is at most 2^30; not below -1: no difference wraps
     int last = pos;
 #pragma unroll
@@ -473,7 +477,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     for (int x = tid; x < kA8Rows * HD / 8; x += kA8Threads) {
         const int r = x / (HD / 8), d = (x % (HD / 8)) * 8;
         const int rt = r / a.rows_heads, rh = ht * a.rows_heads + r % a.rows_heads;
-        if (rt >= n || rh >= a.group) continue;
+        if (!(s_live >> (4 * r) & 1)) continue;
         float m = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kA8Warps; ++w) m = fmaxf(m, s_m[w][r]);
@@ -508,7 +512,7 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     for (int x = chunk * kA8Threads + tid; x < kA8Rows * HD / 4; x += a.n_chunks * kA8Threads) {
         const int r = x / (HD / 4), d = (x % (HD / 4)) * 4;
         const int rt = r / a.rows_heads, rh = ht * a.rows_heads + r % a.rows_heads;
-        if (rt >= n || rh >= a.group) continue;
+        if (!(s_live >> (4 * r) & 1)) continue;
         float mp[kA8MaxCluster], lp[kA8MaxCluster], m = -INFINITY;
         float4 v[kA8MaxCluster];
 #pragma unroll
@@ -557,7 +561,9 @@ __global__ void __launch_bounds__(128) k_attn_kv8_join(const Attn8Args a) {
         last = min(first + a.rows_toks, end) - 1;
     }
     int lp = -1;
-    for (int i = first; i <= last; ++i) lp = max(lp, a.tok_pos[i]);
+    for (int i = first + lane; i <= last; i += 32)               // every warp for itself
+        if (a.tok_seq[i] == seq) lp = max(lp, a.tok_pos[i]);
+    lp = __reduce_max_sync(0xffffffffu, lp);
     lp = (int)min((long long)lp, (long long)a.width * kPage - 1);
     const int chunks = attn8_chunks(a, lp);
     if (chunks <= 1) return;

@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
     }
     // last position of each tile's tokens
     if (tid < 2 * kT8Rows) {
-        const int pos = tid < n ? max(min(a.tok_pos[t0 + tid], most), -1) : -1;
+        const int pos = tid < n && a.tok_seq[t0 + tid] == seq ? max(min(a.tok_pos[t0 + tid], most), -1) : -1;
         const int p0 = __reduce_max_sync(0xffffffffu, tid < toks ? pos : -1), p1 = __reduce_max_sync(0xffffffffu, tid < toks ? -1 : pos);
         if (lane == 0) { s_last[0][warp] = p0; s_last[1][warp] = p1; }
     }
@@ -402,6 +402,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
         const int tile = warp >> 2, r = tid & 127;
         int pos = 0, row_tok = -1, row_head = 0;
         if (r / group < toks && tile * toks + r / group < n) { row_tok = t0 + tile * toks + r / group; row_head = head * group + r % group; }
+        if (row_tok >= 0 && a.tok_seq[row_tok] != seq) row_tok = -1;         // an entry that does not belong to the sequence is skipped
         pos = row_tok >= 0 ? max(min(a.tok_pos[row_tok], most), -1) - key0 : -1;      // tok_pos may be anything: a difference must not wrap
         {
             constexpr int CH = HD / 8, RPI = 32 / CH;          // lanes per row, rows at a time
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t o_at = lanes + NT * 2 * kT8Keys + tile * HD;
         const int my_steps = tile ? n1 : n0;
-        const int open = row_tok >= 0 ? pos : 0x7fffffff;      // rows of no token: q = 0, whatever they come to is not written
+        const int open = row_tok >= 0 ? pos : 0x7fffffff;      // rows of no token, or of one that is skipped: whatever they come to is not written
         const int all_see = __reduce_min_sync(0xffffffffu, open);
         float m = -INFINITY, l = 0.f, vr = 0.f;
         // One step: the 64 scores of a row stay in registers.

@@ -44,6 +44,28 @@ def test_tables_of_many_pages(dtype, h, grp, d):
         check_attention(a, dtype, keys=4040, **kw)
 
 
+@pytest.mark.parametrize("h,grp,d", [(1, 1, 64), (2, 4, 128), (1, 8, 64), (1, 2, 16)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_entries_of_no_sequence_inside_a_run(dtype, h, grp, d):
+    """With cu_tok too an entry whose tok_seq names no sequence, or another than the one in whose run it stands, is skipped and its row left
+    as it was, however the keys are cut; the others are as if it attended nothing."""
+    for before, new, lens in (([700, 0], [12, 5], (712, 0, 50)), ([9000, 3], [70, 64], (9070, 1500)), ([300, 20, 0], [140, 2, 200], (440,)), ([2000], [3], (2003,))):
+        a = setup_attention(before, new, h, grp, d, dtype, seed=6)
+        q, pages, scales, table, seq, pos, cu = a
+        odd = {1: -1, 2: len(new), 5: -2 ** 31, 11: 1 if len(new) > 1 else -1, new[0] - 1: 2 ** 31 - 1}
+        for max_len in lens:
+            for max_new in (max(new), 2, 0):
+                mixed = seq.clone()
+                for t, s in odd.items():
+                    if t < new[0]:
+                        mixed[t] = s
+                gone = mixed != seq
+                want = kv8.attention(q, pages, scales, table, seq, pos.masked_fill(gone, -1), cu, max_new=max_new, max_len=max_len)
+                got = kv8.attention(q, pages, scales, table, mixed, pos, cu, max_new=max_new, max_len=max_len, out=torch.full_like(q, 3.0))
+                assert bool((got[gone] == 3.0).all())
+                assert torch.equal(got[~gone], want[~gone])
+
+
 def test_paged_cache_says_what_attention_found():
     cache = kv8.PagedCache(1, 2, 8, 2, 64, max_len=200, max_tok=130)
     cache.step(torch.tensor([100, 30], dtype=torch.int32, device="cuda"))
