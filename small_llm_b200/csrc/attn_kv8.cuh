@@ -229,10 +229,11 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
         for (int i = 0; i < KB; ++i) top = fmaxf(top, fabsf(x[i]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // f = 2^-e with top in [2^(e-1), 2^e): exponents are kept where f and 1 / f are normal numbers
-        const int e = min(max((int)(__float_as_uint(top) >> 23) - 126, -125), 125);
-        const float f = top > 0.f ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
-        row_f = (top > 0.f ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f) * a.scale * 1.4426950408889634f;
+        // f = 2^(h - e) with top in [2^(e-1), 2^e), and its inverse: with h both are normal numbers up to the largest e, and the
+        // low fp16 parts good to 2^-39 of the largest value
+        const int e = min(max((int)(__float_as_uint(top) >> 23) - 126, -125), 128), h = e > -100 ? 14 : 0;
+        const float f = top > 0.f ? __uint_as_float((uint32_t)(127 + h - e) << 23) : 1.f;
+        row_f = (top > 0.f ? __uint_as_float((uint32_t)(127 + e - h) << 23) : 1.f) * a.scale * 1.4426950408889634f;
         if constexpr (I8) {
             // digits know no infinity and no NaN: the row's factor carries them
             float odd = 0.f;
@@ -240,14 +241,15 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
             for (int i = 0; i < KB; ++i) odd = fmaf(x[i], 0.f, odd);
             odd += __shfl_xor_sync(0xffffffffu, odd, 1);
             odd += __shfl_xor_sync(0xffffffffu, odd, 2);
-            row_f = row_f * (1.f / kDigits) + odd;
-            const float fd = row_ok ? f * kDigits : 0.f;
+            row_f = row_f * (h ? 16384.f / kDigits : 1.f / kDigits) + odd;
+            const float fd = h ? kDigits / 16384.f : kDigits;            // f * fd may be no number of fp32: q is multiplied by one after the other
+            const float f_ok = row_ok ? f : 0.f;
 #pragma unroll
             for (int j = 0; j < KS; ++j)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float* y = x + 8 * j + 4 * h;
-                    digits4(digit_bits(y[0], fd), digit_bits(y[1], fd), digit_bits(y[2], fd), digit_bits(y[3], fd), qa[j][2 * h], qa[j][2 * h + 1]);
+                for (int i = 0; i < 2; ++i) {
+                    const float* y = x + 8 * j + 4 * i;
+                    digits4(digit_bits(y[0] * f_ok, fd), digit_bits(y[1] * f_ok, fd), digit_bits(y[2] * f_ok, fd), digit_bits(y[3] * f_ok, fd), qa[j][2 * i], qa[j][2 * i + 1]);
                 }
         } else
 #pragma unroll

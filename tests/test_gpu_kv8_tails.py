@@ -11,7 +11,7 @@ import torch
 
 from small_llm_b200 import kv8
 
-from .test_gpu_kv8 import BLOCK, PAGE, ceil, gen
+from .test_gpu_kv8 import BLOCK, PAGE, ceil, check_attention, gen, setup_attention
 
 pytestmark = pytest.mark.gpu
 UNIT = 32                                        # keys whose weights the general form takes relative to their own largest
@@ -138,3 +138,18 @@ def test_values_near_the_largest_number(dtype, d):
     i32 = dict(dtype=torch.int32, device="cuda")
     got = kv8.attention(torch.ones(1, 1, d, dtype=dtype, device="cuda"), pages, scales, torch.zeros(1, 1, **i32), torch.zeros(1, **i32), torch.ones(1, **i32), max_new=1)
     assert bool(((got.double() / (95.5 * 2.0 ** 119) - 1).abs() <= (2.0 ** -8 + 2.0 ** -15 if dtype == torch.bfloat16 else 2.0 ** -20)).all())
+
+
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_queries_near_the_largest_and_the_smallest_number(dtype, d):
+    """Query values up to the type's largest, and near its smallest normal one, under a softmax scale that undoes them."""
+    for size, scale in ((torch.finfo(dtype).max, 1.2e-38), (2.0 ** -120, 2.0 ** 118)):
+        q, pages, scales, table, seq, pos, cu = setup_attention([300, 40], [60, 60], 1, 2, d, dtype, seed=24)
+        scales[:, :, 0] *= 0.25
+        x = torch.rand(q.shape, device="cuda", generator=gen(25)) * 2 - 1
+        x[:, :, 3] = torch.sign(x[:, :, 3])
+        q = (x.double() * size).to(dtype)
+        assert bool(torch.isfinite(q).all())
+        for kw in (dict(max_new=1), dict(cu_tok=cu)):
+            check_attention((q, pages, scales, table, seq, pos, cu), dtype, scale=scale, max_len=360, **kw)
