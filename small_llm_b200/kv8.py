@@ -182,7 +182,7 @@ def attention(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, table:
         out = torch.empty((n, heads, d), dtype=q.dtype, device=q.device)
     _need(out.dtype is q.dtype, "out must have q's dtype")
     _need(0 <= max_new < 1 << 31 and 0 <= max_len < 1 << 31, "max_new and max_len must not be negative")
-    _need(scale is None or scale != 0, "scale must not be 0")
+    _need(scale is None or 1.5e-45 < abs(scale) < 3.4e38, "scale must be a finite number other than 0 in fp32")      # as a float 0 it would mean the default
     a = _pack_attn(q.data_ptr(), out.data_ptr(), q_stride, _rows("out", out, n, heads, d, dev), _flat("table", table, _I32, (n_seq, width), dev),
                    _flat("tok_seq", tok_seq, _I32, (n,), dev), _flat("tok_pos", tok_pos, _I32, (n,), dev),
                    0 if cu_tok is None else _flat("cu_tok", cu_tok, _I32, (n_seq + 1,), dev), 0 if status is None else _flat("status", status, _I32, (1,), dev),

@@ -79,3 +79,13 @@ def test_paged_cache_says_what_attention_found():
     mine = torch.zeros(1, dtype=torch.int32, device="cuda")
     cache.attention(0, x, status=mine)
     assert int(mine) == 1 and cache.status() == 0
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-46, -1e-60, 1e39, float("inf"), float("-inf"), float("nan")])
+def test_softmax_scales_that_fp32_does_not_have(scale):
+    """One that fp32 rounds to 0 would stand for the default scale."""
+    q, pages, scales, table, seq, pos, cu = setup_attention([40], [1], 1, 1, 64, torch.float32, seed=9)
+    with pytest.raises(ValueError, match="scale"):
+        kv8.attention(q, pages, scales, table, seq, pos, scale=scale)
+    tiny = kv8.attention(q, pages, scales, table, seq, pos, scale=1e-44)      # the smallest ones count: all keys alike
+    assert float((tiny - kv8.attention(q * 0, pages, scales, table, seq, pos)).abs().max()) < 1e-5
