@@ -5,7 +5,7 @@ import torch
 
 from small_llm_b200 import kv8
 
-from .test_gpu_kv8 import TYPES, check_attention, setup_attention
+from .test_gpu_kv8 import BLOCK, PAGE, TYPES, check_attention, gen, setup_attention
 
 pytestmark = pytest.mark.gpu
 LOWEST = -2 ** 31
@@ -89,3 +89,35 @@ def test_softmax_scales_that_fp32_does_not_have(scale):
         kv8.attention(q, pages, scales, table, seq, pos, scale=scale)
     tiny = kv8.attention(q, pages, scales, table, seq, pos, scale=1e-44)      # the smallest ones count: all keys alike
     assert float((tiny - kv8.attention(q * 0, pages, scales, table, seq, pos)).abs().max()) < 1e-5
+
+
+def test_tokens_appended_one_at_a_time():
+    """What a decode loop's cache stands for, against the rows themselves: each rounding of a row, under its first scale and under every
+    scale that the block grew to while it held it, is off by half a step at most; and over many rows the root of the mean square is no
+    more than that many independent roundings would leave."""
+    n, h, d = 32 * BLOCK, 2, 64
+    k, v = torch.randn(2, n, h, d, device="cuda", generator=gen(41))
+    slots = torch.arange(n, device="cuda")
+    pages, scales = kv8.empty_cache(n // PAGE, h, d)
+    seen = torch.zeros(2, n, h, dtype=torch.float64, device="cuda")          # sum over the roundings of a row: half a step
+    square = torch.zeros_like(seen)                                          # the same of step^2 / 12
+    block = lambda t: scales[t // PAGE, :, :, t % PAGE // BLOCK].double().T  # noqa: E731
+    for t in range(n):
+        first = t % BLOCK == 0
+        was = block(t).clone()
+        kv8.append(k[t:t + 1], v[t:t + 1], slots[t:t + 1], pages, scales)
+        now = block(t)
+        assert first or bool((now >= was).all())
+        for i in range(t // BLOCK * BLOCK, t + 1):
+            moved = torch.ones_like(now) if i == t else (now != was).double()
+            seen[:, i] += moved * now / 2
+            square[:, i] += moved * now ** 2 / 12
+    got = torch.stack(kv8.read(slots, pages, scales))
+    err = got.double() - torch.stack([k, v]).double()
+    assert bool((err.abs() <= seen[..., None] * (1 + 2.0 ** -20)).all())
+    # 2 x 512 x 2 x 64 errors, nearly independent: the mean of their squares is known to better than 2 %
+    assert float((err ** 2).mean()) <= 1.05 * float(square.mean())
+    whole_p, whole_s = kv8.empty_cache(n // PAGE, h, d)                      # one call for all: rounded once
+    kv8.append(k, v, slots, whole_p, whole_s)
+    assert torch.equal(whole_s, scales)                                      # the scales do not depend on the cut, the integers do
+    assert not torch.equal(whole_p, pages)
