@@ -198,11 +198,13 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
     const int chunk = blockIdx.z;
     // this lane's row
     const int r_tok = g / a.rows_heads, r_head = ht * a.rows_heads + g % a.rows_heads;
-    // a list's entry in a sequence's place that does not say so is skipped (without cu_tok the sequence is its own)
-    const bool row_ok = r_tok < n && r_head < a.group && (!a.cu_tok || a.tok_seq[t0 + r_tok] == seq);
+    // an entry in a sequence's run that does not name it is skipped (without cu_tok the entry has named its sequence); both loads at once
+    int who = -1, at = -1;
+    if (r_tok < n && r_head < a.group) { at = a.tok_pos[t0 + r_tok]; who = a.cu_tok ? a.tok_seq[t0 + r_tok] : seq; }
+    const bool row_ok = who == seq;
     const unsigned rows = __ballot_sync(0xffffffffu, row_ok);
     if (tid == 0) s_live = rows;
-    const int pos = row_ok ? max(min(a.tok_pos[t0 + r_tok], a.width * kPage - 1), -1) : -1;      // width * 64 is at most 2^30; not below -1: no difference wraps
+    const int pos = row_ok ? max(min(at, a.width * kPage - 1), -1) : -1;      // width * 64 is at most 2^30; not below -1: no difference wraps
     int last = pos;
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));

@@ -209,7 +209,9 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
     }
     // last position of each tile's tokens
     if (tid < 2 * kT8Rows) {
-        const int pos = tid < n && a.tok_seq[t0 + tid] == seq ? max(min(a.tok_pos[t0 + tid], most), -1) : -1;
+        int who = -1, at = -1;
+        if (tid < n) { who = a.tok_seq[t0 + tid]; at = a.tok_pos[t0 + tid]; }
+        const int pos = who == seq ? max(min(at, most), -1) : -1;            // an entry that does not name the sequence is skipped
         const int p0 = __reduce_max_sync(0xffffffffu, tid < toks ? pos : -1), p1 = __reduce_max_sync(0xffffffffu, tid < toks ? -1 : pos);
         if (lane == 0) { s_last[0][warp] = p0; s_last[1][warp] = p1; }
     }
@@ -400,10 +402,11 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
         // This thread's row; and the warp's 32 rows of q as fp16, K-major with the 128-byte swizzle, read and written by HD / 8 lanes each.
         // Rows of no token are zero.
         const int tile = warp >> 2, r = tid & 127;
-        int pos = 0, row_tok = -1, row_head = 0;
-        if (r / group < toks && tile * toks + r / group < n) { row_tok = t0 + tile * toks + r / group; row_head = head * group + r % group; }
-        if (row_tok >= 0 && a.tok_seq[row_tok] != seq) row_tok = -1;         // an entry that does not belong to the sequence is skipped
-        pos = row_tok >= 0 ? max(min(a.tok_pos[row_tok], most), -1) - key0 : -1;      // tok_pos may be anything: a difference must not wrap
+        int pos = -1, row_tok = -1, row_head = 0;
+        if (r / group < toks && tile * toks + r / group < n) {
+            const int at = t0 + tile * toks + r / group, p = a.tok_pos[at];
+            if (a.tok_seq[at] == seq) { row_tok = at; row_head = head * group + r % group; pos = max(min(p, most), -1) - key0; }     // tok_pos may be anything: no difference wraps
+        }
         {
             constexpr int CH = HD / 8, RPI = 32 / CH;          // lanes per row, rows at a time
             const int c = lane % CH;
