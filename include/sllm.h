@@ -296,7 +296,11 @@ int sllm_k_kv8_read(const sllm_kv8_layer* c, const sllm_kv8_rows* r, void* strea
 
 /* Causal attention over the cache: token t, of sequence tok_seq[t], attends the positions 0 .. tok_pos[t] of that sequence
  * (its own included: append first).  n_heads is a multiple of kv_heads; query head h attends kv head h / (n_heads / kv_heads).
- * Softmax in fp32 and the integers of the cache exactly; fp32 rows keep fp32 accuracy.
+ * Softmax and sums in fp32 and the integers of the cache exactly; fp32 rows keep fp32 accuracy.  bf16 rows: a query row's values enter
+ * to 2^-17 of its largest and a weight (times its block's scale of V) to 2^-16 of the largest of 32 keys; in the form for
+ * prompts a query row's values enter exactly down to 2^-16 of its largest and a weight to 2^-11 of itself or 2^-32 of the row's largest,
+ * whichever is more; all of it is less than the rounding of the output.  That form takes a
+ * sequence's scales of V within 2^-60 and 2^100 of those of its first page.  A scale that is not finite makes the rows that attend its block NaN.
  * A token with tok_seq outside 0 .. n_seq - 1 is skipped, its output row left as it was; one with tok_pos < 0 gets zeros.  A
  * page outside the pool is not attended.  *status (when given, an int32 that the call never clears) becomes SLLM_ERR_INVALID when
  * there was one, and SLLM_ERR_DEVICE_WAIT when a bounded wait of a kernel gave up.  The rows that such a wait concerns are NaN, with
@@ -304,7 +308,7 @@ int sllm_k_kv8_read(const sllm_kv8_layer* c, const sllm_kv8_rows* r, void* strea
  * max_new: the most entries that one sequence has; max_len: the most positions that one has.  They choose between kernels and how
  * the keys are cut; 0 = not known; a wrong value costs time, not results.  cu_tok (NULL allowed: then every token is taken
  * alone) says that entries cu_tok[i] .. cu_tok[i + 1] - 1 are sequence i's, with the table's row i; it is used when max_new != 1, and
- * entries whose tok_seq is not i are then skipped as well. */
+ * entries outside these runs, or whose tok_seq is not i, are then skipped as well. */
 typedef struct {
     const void* q;                            /* [n_tok], rows of n_heads * head_dim elements                      */
     void* out;                                /* the same; may not overlap q                                       */

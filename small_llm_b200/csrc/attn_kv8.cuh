@@ -23,9 +23,12 @@
 // two units ahead, and has its own running state; the states are joined once.  Keys are cut into chunks when there are few
 // rows: of a few short rows at most eight, the blocks of a cluster, which join their states through one another's shared memory;
 // otherwise the states go to the workspace, and a second, small kernel joins them.
-// Measured (of the 6460 GB/s of a copy): 512 sequences of 256 to 2047 positions, ten heads of 64, 127 us = 6.0 TB/s; four of 60 to 131
-// thousand, 8 kv heads of 128 with four query heads each, 138 us = 5.7 TB/s; one of 2048, ten heads, 7 us, which is latency: the
-// lists, the table, the pages, the join.  With fp16 products for bf16 rows too the first took 178 us, bound by instruction issue.
+// Measured (of the 6460 GB/s of a copy; the kernel repeated in a graph, and with caches that other passes have left cold): 512 sequences of
+// 256 to 2047 positions, ten heads of 64, 124 and 142 us = 6.2 and 5.4 TB/s; four of 60 to 131
+// thousand, 8 kv heads of 128 with four query heads each, 138 and 147 us = 5.7 and 5.4 TB/s; one of 2048, ten heads, 7 us, which is latency: the
+// lists, the table, the pages, the join.  With fp16 products for bf16 rows too the first took 178 us, bound by instruction issue.  A running
+// reference for all units' weights and 32-bit integer accumulators, which a strong key leaves too few bits, took 127 us: 96
+// registers and not 80, five blocks per SM and not six.
 #pragma once
 #include <cuda_fp16.h>
 
