@@ -297,7 +297,7 @@ int sllm_k_kv8_read(const sllm_kv8_layer* c, const sllm_kv8_rows* r, void* strea
 /* Causal attention over the cache: token t, of sequence tok_seq[t], attends the positions 0 .. tok_pos[t] of that sequence
  * (its own included: append first).  n_heads is a multiple of kv_heads; query head h attends kv head h / (n_heads / kv_heads).
  * Softmax and sums in fp32 and the integers of the cache exactly; fp32 rows keep fp32 accuracy.  bf16 rows: a query row's values enter
- * to 2^-17 of its largest and a weight (times its block's scale of V) to 2^-16 of the largest of 32 keys; in the form for
+ * exactly down to 2^-6 of its largest, or to 2^-15 of that, and a weight (times its block's scale of V) to 2^-16 of the largest of 32 keys; in the form for
  * prompts a query row's values enter exactly down to 2^-16 of its largest and a weight to 2^-11 of itself or 2^-32 of the row's largest,
  * whichever is more; all of it is less than the rounding of the output.  That form takes a
  * sequence's scales of V within 2^-60 and 2^100 of those of its first page.  A scale that is not finite makes the rows that attend its block NaN.

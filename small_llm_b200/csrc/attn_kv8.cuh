@@ -11,9 +11,9 @@
 // relative to their own largest, and the unit's sum is added, with that factor, to an fp32 accumulator relative to m.  So the
 // precision of a weight is that of its unit: neither the loudest value of the cache, nor a strong key (an attention sink) elsewhere
 // in it, takes bits from what many small weights add up to.  Two forms:
-//   bf16 rows (I8): m16n8k32 on int8, the cache's bytes as they are.  q and p vs become two base-256 digits, 16 bits in all: q
-//     to 2^-17 of the row's largest value (bf16 has 2^-9 of each), p vs to 2^-16 of the unit's largest (the
-//     output is rounded to 2^-9).  Products and a unit's sums are exact, in 32-bit integers.
+//   bf16 rows (I8): m16n8k32 on int8, the cache's bytes as they are.  q and p vs become two base-256 digits, 16 bits in all: q, multiplied
+//     by a power of two, exactly down to 2^-7 of the row's largest value (2^-6 where its bits are all ones) and to 2^-15 of that below, p vs to
+//     2^-16 of the unit's largest (the output is rounded to 2^-9).  Products and a unit's sums are exact, in 32-bit integers.
 //   fp32 rows: m16n8k16 on fp16, in which the integers are exact, q and p vs split into a high and a low fp16 part, 22 bits (p vs to 2^-39
 //     of the unit's largest at least), fp32 sums: fp32 accuracy.  A byte costs 1.25-1.5 instructions on its way there (xor the sign, byte-permute under 0x64
 //     = 1024 + x, subtract), where I8 spends none on K and half of one on V, to bring four keys of a dim into one register.
@@ -79,8 +79,8 @@ __device__ __forceinline__ void mma16832(int (&c)[4], const uint32_t (&a)[4], ui
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Four values in [-1, 1] times 32512, rounded, as two base-256 digits each: the high ones in [-127, 127], the low ones in
-// [-128, 127].  The sum with 1.5 * 2^23 + 128 leaves the integer, 128 up, in the low bits: its second byte is the high digit and
+// Four values times a factor, at most 32639 and rounded, as two base-256 digits each: the high ones in [-127, 127], the low ones in
+// [-128, 127].  (Weights, in [0, 1], times 32512.)  The sum with 1.5 * 2^23 + 128 leaves the integer, 128 up, in the low bits: its second byte is the high digit and
 // its first, sign flipped, the low one.
 constexpr float kDigits = 32512.f;
 constexpr float kSplitTop = 16384.f;   // what a unit's largest weight of the fp16 form is brought to: its parts are then good to 2^-39 of it
@@ -235,8 +235,9 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // f = 2^(h - e) with top in [2^(e-1), 2^e), and its inverse: with h both are normal numbers up to the largest e, and the
-        // low fp16 parts good to 2^-39 of the largest value
-        const int e = min(max((int)(__float_as_uint(top) >> 23) - 126, -125), 128), h = e > -100 ? 14 : 0;
+        // low fp16 parts good to 2^-39 of the largest value.  Digits are of q 2^(15 - e): a bf16 top whose bits are all ones, which would
+        // pass 127 * 256 + 127 there, counts as the next power of two.
+        const int e = min(max((int)((__float_as_uint(top) + (I8 ? 0x10000u : 0u)) >> 23) - 126, -125), 129), h = e > -100 ? 14 : 0;
         const float f = top > 0.f ? __uint_as_float((uint32_t)(127 + h - e) << 23) : 1.f;
         row_f = (top > 0.f ? __uint_as_float((uint32_t)(127 + e - h) << 23) : 1.f) * a.scale * 1.4426950408889634f;
         if constexpr (I8) {
@@ -246,8 +247,8 @@ __global__ void __launch_bounds__(kA8Threads) k_attn_kv8(const Attn8Args a) {
             for (int i = 0; i < KB; ++i) odd = fmaf(x[i], 0.f, odd);
             odd += __shfl_xor_sync(0xffffffffu, odd, 1);
             odd += __shfl_xor_sync(0xffffffffu, odd, 2);
-            row_f = row_f * (h ? 16384.f / kDigits : 1.f / kDigits) + odd;
-            const float fd = h ? kDigits / 16384.f : kDigits;            // f * fd may be no number of fp32: q is multiplied by one after the other
+            row_f = row_f * (h ? 0.5f : 1.f / 32768.f) + odd;
+            const float fd = h ? 2.f : 32768.f;          // f * fd may be no number of fp32: q is multiplied by one after the other
             const float f_ok = row_ok ? f : 0.f;
 #pragma unroll
             for (int j = 0; j < KS; ++j)

@@ -153,3 +153,32 @@ def test_queries_near_the_largest_and_the_smallest_number(dtype, d):
         assert bool(torch.isfinite(q).all())
         for kw in (dict(max_new=1), dict(cu_tok=cu)):
             check_attention((q, pages, scales, table, seq, pos, cu), dtype, scale=scale, max_len=360, **kw)
+
+
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scores_of_hundreds(dtype, d):
+    """Two keys of nearly the same large score, which the query reaches by different values, 129 / 256 and 131 / 256 beside a largest of 1:
+    a rounding of the query in steps that are not a power of two moves the scores apart."""
+    a, b = d // 2 * 100 * 129, (d // 2 - 1) * 131
+    kb = round(a / b)
+    q = torch.full((1, 1, d), 131 / 256, device="cuda")
+    q[..., 1::2], q[..., 0] = 129 / 256, 1.0
+    pages, scales = kv8.empty_cache(1, 1, d)
+    pages[0, 0, 0, 0, 1::2], pages[0, 0, 0, 1, 2::2] = 100, kb
+    pages[0, 0, 1, 0], pages[0, 0, 1, 1] = 127, -127
+    scales[0, 0, 0], scales[0, 0, 1] = 400 * 256 * d ** 0.5 / a, 1 / 127
+    i32 = dict(dtype=torch.int32, device="cuda")
+    args = (q.to(dtype), pages, scales, torch.zeros(1, 1, **i32), torch.zeros(1, **i32), torch.ones(1, **i32), torch.tensor([0, 1], **i32))
+    for kw in (dict(max_new=1), dict(cu_tok=args[6])):
+        check_attention(args, dtype, **kw)
+
+
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_random_scores_of_hundreds(dtype, d):
+    """Scores so large that a rounding of the queries themselves, beyond their type's, would show in the weights."""
+    q, pages, scales, table, seq, pos, cu = setup_attention([300, 40, 131, 200, 77, 260], [1] * 6, 2, 64, d, dtype, seed=26, sharp=6.0)
+    scales[:, :, 0] *= 8
+    for kw in (dict(max_new=1), dict(cu_tok=cu)):
+        check_attention((q, pages, scales, table, seq, pos, cu), dtype, max_len=301, **kw)
