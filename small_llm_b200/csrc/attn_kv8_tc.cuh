@@ -513,8 +513,8 @@ __global__ void __launch_bounds__(attn8_tc_threads<NT>(), NT == 1 ? 2 : 1) k_att
                 l_add = 0.f;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    // c stays above zero so that -inf stays -inf; a block behind the row does not count, whatever it holds: S is -inf there,
-                    // and f.y, which alone may be NaN, is not used
+                    // c stays above zero, also beside a NaN, so that -inf stays -inf; a block behind the row does not count, whatever it holds: S
+                    // is -inf there, and f.y, by which a scale that is not finite comes, is not used
                     const float4 f = blk[b];
                     const bool behind = k0 + b * 16 > open;
                     const float c = fmaxf(f.x * row_f, 1e-37f), d = behind ? -INFINITY : f.y - m_use;
